@@ -330,6 +330,51 @@ int rwkvb200_wkv6_bwd_varlen(const void* r, const void* k, const void* v, const 
 
 
 /* ------------------------------------------------------------------------------------------
+ * Linear attention with a decay for each head (no counterpart in the reference).  Per (sequence, head):
+ *   S_t = exp(-exp(w_t)) S_{t-1} + v_t k_t^T        o_t = S_t r_t        S [V][K], float32
+ *   r, k, v, o   [B][T][H][D] ([B][H][T][D] when head_first), or with seq_start / seq_len (device arrays, n_seq entries)
+ *                packed in one row [1][total][H][D]; then n_seq counts the sequences, max_len is the longest length, and rows
+ *                of no sequence are neither read into a result nor written.  Dense: n_seq = B, max_len = T, total ignored.
+ *   w            float32: one number per head [H] (w_per_head) or per token and head, laid out like the tokens without D
+ *   head size    64 or 128
+ *   h0           float32 [n_state][H][D][D], n_state 0 (none: zero), 1 (shared) or n_seq;  ht [n_seq][H][D][D], may be NULL
+ *   states       rwkvb200_linattn_states_bytes(..., keep = 1) of memory in which the forward leaves the states that the backward starts from; a
+ *                forward without a backward passes keep = 0 and that much (possibly none).  o NULL: the states alone.
+ * Backward: gradients of r, w (like w, float32), k, v and of the state each sequence started from (dh0 [n_seq][H][D][D], may be NULL);
+ * d_ht may be NULL (zero).  workspace: rwkvb200_linattn_workspace_bytes (total 0 for a dense batch).
+ * rwkvb200_linattn_step: one token in place on resident states [groups * beams][H][D][D], float32 or bfloat16; with parents
+ *   [groups][beams] sequence j of a group goes on from the state of sequence parents[j] of that group (at most 32 beams).
+ * rwkvb200_reorder_states: the same reordering alone, in place, for rows of any `row_bytes` (a multiple of 16) [groups][beams]; rows that
+ *   stay are not touched.  Entries of parents outside [0, beams) are clamped.
+ * ---------------------------------------------------------------------------------------- */
+size_t rwkvb200_linattn_states_bytes(int n_seq, int max_len, int H, int head_size, int dtype, int keep);
+size_t rwkvb200_linattn_workspace_bytes(int n_seq, int max_len, int total, int H, int head_size, int dtype, int w_per_head, int backward);
+int rwkvb200_linattn_fwd(const void* r, const float* w, int w_per_head, const void* k, const void* v,
+                         const float* h0, int n_state, void* o, float* ht, float* states, size_t states_bytes,
+                         void* workspace, size_t workspace_bytes, const int32_t* seq_start, const int32_t* seq_len,
+                         int n_seq, int max_len, int total, int H, int head_size, int dtype, int head_first, void* stream);
+int rwkvb200_linattn_bwd(const void* r, const float* w, int w_per_head, const void* k, const void* v, const void* d_o,
+                         const float* d_ht, const float* states, size_t states_bytes,
+                         void* dr, float* dw, void* dk, void* dv, float* dh0, void* workspace, size_t workspace_bytes,
+                         const int32_t* seq_start, const int32_t* seq_len,
+                         int n_seq, int max_len, int total, int H, int head_size, int dtype, int head_first, void* stream);
+int rwkvb200_linattn_step(const void* r, const float* w, int w_per_head, const void* k, const void* v,
+                          void* state, int state_dtype, void* o, const int64_t* parents, int groups, int beams,
+                          int H, int head_size, int dtype, void* stream);
+int rwkvb200_reorder_states(void* state, const int64_t* parents, int groups, int beams, size_t row_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Beam search (no counterpart in the reference): the best continuations of `groups` searches of `beams` (at most 32) beams over
+ * `vocab` tokens.  Candidate (i, t) of a group has the score scores[i] + logits[i][t] - log sum_u exp(logits[i][u]); the `beams` best are
+ * returned in descending order, ties to the lowest i * vocab + t.  A beam marked in `finished` (may be NULL) goes on with eos alone,
+ * at the score it has.  finished_out (may be NULL): whether the parent had finished or the token is eos.  eos < 0: none.
+ * logits: last dimension contiguous, strides in elements; NaN and +inf count as -inf.
+ * ---------------------------------------------------------------------------------------- */
+int rwkvb200_beam_select(const void* logits, int dtype, int64_t group_stride, int64_t beam_stride, const float* scores,
+                         const uint8_t* finished, int64_t eos, float* scores_out, int64_t* parents, int64_t* tokens,
+                         uint8_t* finished_out, int groups, int beams, int vocab, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Diagnostics of the tensor-core path (no counterpart in the reference).
  * rwkvb200_device_status: every wait inside a tensor-core kernel (on an mbarrier that a TMA copy or
  *   an MMA completes) gives up after a fixed number of polls, records a non-zero code in a status word

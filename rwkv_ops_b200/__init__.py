@@ -7,13 +7,17 @@ variables of the reference are not consulted: there is one implementation, hand-
 behind a C ABI, and it raises if its shared library is missing.  ``Rwkv7DecodeState`` (in-place
 single-token decoding) ``generalized_delta_rule_varlen`` / ``wkv6_varlen`` (packed variable-length batches) and
 ``generalized_delta_rule_fused`` (the producers of w, a, b computed inside the operator) go beyond the
-reference's working surface.
+reference's working surface, and so do linear attention with a decay for each head (``linear_attention``,
+``linear_attention_varlen``, ``LinearAttentionDecodeState``) and beam search over resident states (``beam_select``,
+``reorder_states``).
 """
 from .rwkv7 import generalized_delta_rule, get_generalized_delta_rule
 from .rwkv6 import RWKVKernelOperator, get_rwkv6_kernel
 from .decode import Rwkv7DecodeState
 from .varlen import PackedSequences, generalized_delta_rule_varlen, wkv6_varlen
 from .fused import generalized_delta_rule_fused
+from .linear_attention import LinearAttentionDecodeState, linear_attention, linear_attention_varlen, reorder_states
+from .beam import beam_select
 
 from . import _ops
 
@@ -42,4 +46,9 @@ __all__ = [
     "PackedSequences",
     "wkv6_varlen",
     "generalized_delta_rule_fused",
+    "linear_attention",
+    "linear_attention_varlen",
+    "LinearAttentionDecodeState",
+    "reorder_states",
+    "beam_select",
 ]

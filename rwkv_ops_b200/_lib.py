@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_int, c_size_t, c_void_p, c_char_p
+from ctypes import c_int, c_int64, c_size_t, c_void_p, c_char_p
 
 import torch
 
@@ -58,6 +58,13 @@ SIGNATURES = {
     "rwkvb200_wkv6_fwd_varlen": (c_int, [_P] * 5 + [_P, _P, _I, _I, _I, _P, _I, _P, _P, _P, _P, _Z] + [_I] * 4 + [_P]),
     "rwkvb200_wkv6_bwd_varlen": (c_int, [_P] * 5 + [_P, _P, _I, _I, _I, _P, _I, _P, _P, _P] + [_P] * 6 + [_P, _Z] +
                                  [_I] * 4 + [_P]),
+    "rwkvb200_linattn_states_bytes": (c_size_t, [_I] * 6),
+    "rwkvb200_linattn_workspace_bytes": (c_size_t, [_I] * 8),
+    "rwkvb200_linattn_fwd": (c_int, [_P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _Z, _P, _Z, _P, _P] + [_I] * 7 + [_P]),
+    "rwkvb200_linattn_bwd": (c_int, [_P, _P, _I] + [_P] * 5 + [_Z] + [_P] * 6 + [_Z, _P, _P] + [_I] * 7 + [_P]),
+    "rwkvb200_linattn_step": (c_int, [_P, _P, _I, _P, _P, _P, _I, _P, _P] + [_I] * 5 + [_P]),
+    "rwkvb200_reorder_states": (c_int, [_P, _P, _I, _I, _Z, _P]),
+    "rwkvb200_beam_select": (c_int, [_P, _I, c_int64, c_int64, _P, _P, c_int64, _P, _P, _P, _P, _I, _I, _I, _P]),
     "rwkvb200_device_status": (c_int, [_I]),
     "rwkvb200_profile_enable": (None, [_I]),
     "rwkvb200_profile_reset": (None, []),
@@ -147,6 +154,13 @@ def wkv6_kept_bytes(B: int, T: int, H: int) -> int:
     nt = (T + 63) // 64
     return (_a256(B * H * (nt + 1) * 64 * 64 * 4) + _a256(B * H * 2 * 64 * 4) + _a256(B * H * 4 * 64 * 4)
             + _a256(B * H * 4) + _a256(B * H * 64 * 64 * 4) + _a256((B * H + 1) * 4))
+
+
+def linattn_states_bytes(n_seq: int, max_len: int, H: int, D: int, dtype: torch.dtype) -> int:
+    """Likewise for ``rwkvb200_linattn_states_bytes(..., keep = 1)``: the states of linear attention before chunks of 128 tokens on the
+    tensor-core path (bfloat16, head size 64), before and after chunks of 64 elsewhere."""
+    chunks = (max_len + 127) // 128 if D == 64 and dtype == torch.bfloat16 else (max_len + 63) // 64 + 1
+    return n_seq * H * chunks * D * D * 4
 
 
 def strerror(code: int) -> str:

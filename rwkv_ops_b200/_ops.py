@@ -118,3 +118,27 @@ def _register_fakes():
     @fake("rwkv_ops_b200::wkv6_bwd_varlen")
     def _(r, k, v, w, u, seq_start, seq_len, max_len, s0, state_map, d_y, d_sT, k_):
         return (*tokens(r, 4), torch.empty_like(u), state(r, seq_start.numel(), *u.shape))
+
+    @fake("rwkv_ops_b200::linattn_fwd")
+    def _(r, w, k, v, seq_start, seq_len, max_len, h0, head_first, keep):
+        B, T, H, D = dims(r, head_first)
+        n, length = (B, T) if seq_start is None else (seq_start.numel(), max_len)
+        return torch.empty_like(r), state(r, n, H, D), kept(r, _lib.linattn_states_bytes(n, length, H, D, r.dtype) if keep else 0)
+
+    @fake("rwkv_ops_b200::linattn_bwd")
+    def _(r, w, k, v, seq_start, seq_len, max_len, h0, d_o, d_ht, k_, head_first):
+        B, T, H, D = dims(r, head_first)
+        return (torch.empty_like(r), torch.empty_like(w), *tokens(r, 2), state(r, B if seq_start is None else seq_start.numel(), H, D))
+
+    @fake("rwkv_ops_b200::linattn_step")
+    def _(r, w, k, v, state, parents):
+        return torch.empty_like(r)
+
+    @fake("rwkv_ops_b200::reorder_states")
+    def _(state, parents):
+        return None
+
+    @fake("rwkv_ops_b200::beam_select")
+    def _(logits, scores, finished, eos):
+        return (torch.empty_like(scores, dtype=torch.float32), *(torch.empty_like(scores, dtype=torch.int64) for _ in range(2)),
+                scores.new_empty(scores.shape if eos >= 0 else (0,), dtype=torch.bool))

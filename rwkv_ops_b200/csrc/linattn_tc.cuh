@@ -1,0 +1,133 @@
+// Linear attention with a decay for each head on tcgen05 (bfloat16 tokens, head size 64): what the forward and backward kernels share.  The
+// equations are in linattn.cuh; a chunk is 128 tokens, so that products over tokens fill the 128 lanes of TMEM and a thread owns a
+// token's row.
+//
+// Precision.  r, k, v, d_o are bfloat16 and enter products as they are.  Operands that carry a decay are split into hi + lo bfloat16 (two products, 2^-17)
+// wherever the result is a state or a gradient of w, which are float32: the keys (queries) that are added to the state (its gradient), and in the backward both
+// states.  A and E are rounded once to bfloat16, as is the state that meets r in the forward: those results are rounded to bfloat16 anyway.
+//
+// Work is cut into items, a stretch of consecutive chunks of one (sequence, head).  With as many units as the device holds CTAs, an item is a unit.  With
+// fewer, a unit is several stretches: a first kernel walks every stretch from a zero state, keys and values only, a small one chains the stretches' states
+// (elementwise), and then all stretches are walked at once from the state each starts with.  That reads half the tokens twice and pays as soon as
+// the chain of chunks is more than a few.
+#pragma once
+
+#include "linattn.cuh"
+#include "tc.cuh"
+
+namespace rwkvb200 {
+namespace la {
+
+using namespace tc;
+typedef __nv_bfloat16 bf16;
+
+constexpr int CT = 128;                        // tokens of a chunk
+constexpr int TOK_BYTES = 2 * TILE_BYTES;      // a chunk of a token tensor: two tiles of 64 tokens x 64 channels
+
+// Decay factors of a chunk.  L is the inclusive prefix sum, Lb(I) its value before the I-th block of 32 tokens; every exponent is a sum over tokens, so
+// every factor is at most one.  A block of 32 x 32 pairs below the diagonal takes its factor e^{L_i - L_j} as row * col, a diagonal one from `in`.
+struct Decays {
+  float start[CT];        // e^{L_i}
+  float end[CT];          // e^{Lc - L_i}
+  float row[CT];          // e^{L_i - Lb(i / 32)}
+  float in[CT], in_lo[CT];      // (L_i - Lb(i / 32)) log2 e, in two floats: under fast decays neighbours differ by little of what has summed up
+  float col[3][CT];       // [I - 1][j]: e^{Lb(I) - L_j}, j < 32 I
+  float all;              // e^{Lc}
+  float pad[3];
+};
+
+// w of a chunk, four consecutive tokens to a lane of one warp.
+struct RawW { float w[4]; };
+__device__ __forceinline__ RawW load_w(const Tokens& t, const float* w, long long wb, int t0, int n) {
+  RawW x;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int i = 4 * (threadIdx.x & 31) + q;
+    x.w[q] = i < n ? __ldg(w + wb + (long long)(t0 + i) * t.wst) : 0.f;
+  }
+  return x;
+}
+// by one warp; tokens from n on do not decay.  g (may be NULL): the tokens' g
+__device__ __forceinline__ void make_decays(Decays& d, const RawW& x, int n, float* g) {
+  const int lane = threadIdx.x & 31;
+  constexpr double LOG2E64 = 1.4426950408889634;
+  double L[4], s = 0.0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const double y = 4 * lane + q < n ? g_of(x.w[q]) : 0.0;
+    if (g) g[4 * lane + q] = (float)y;
+    s += y * LOG2E64;      // all in units of log 2 from here on
+    L[q] = s;
+  }
+  double up = s;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const double y = __shfl_up_sync(0xffffffffu, up, m);
+    if (lane >= m) up += y;
+  }
+  const double before = up - s;      // sums of the lanes before
+#pragma unroll
+  for (int q = 0; q < 4; ++q) L[q] += before;
+  const double Lc = __shfl_sync(0xffffffffu, L[3], 31);
+  const int I = lane >> 3;
+  const double b1 = __shfl_sync(0xffffffffu, L[3], 7), b2 = __shfl_sync(0xffffffffu, L[3], 15), b3 = __shfl_sync(0xffffffffu, L[3], 23);
+  const double mine = I == 0 ? 0.0 : I == 1 ? b1 : I == 2 ? b2 : b3;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int i = 4 * lane + q;
+    d.start[i] = exp2f((float)L[q]);
+    d.end[i] = exp2f((float)(Lc - L[q]));
+    const float in = (float)(L[q] - mine);
+    d.in[i] = in;
+    d.in_lo[i] = (float)(L[q] - mine - (double)in);
+    d.row[i] = exp2f(in);
+    d.col[0][i] = exp2f((float)fmin(b1 - L[q], 0.0));
+    d.col[1][i] = exp2f((float)fmin(b2 - L[q], 0.0));
+    d.col[2][i] = exp2f((float)fmin(b3 - L[q], 0.0));
+  }
+  if (lane == 0) d.all = exp2f((float)Lc);
+}
+
+// The 32 factors of a row of a diagonal block (those above the diagonal mean nothing): e^{L_i - L_j}.
+__device__ __forceinline__ void diagonal_factors(const Decays& d, int row, int first, float (&f)[32]) {
+  const float hi = d.in[row], lo = d.in_lo[row];
+#pragma unroll
+  for (int j = 0; j < 32; j += 4) {
+    const float4 h = *reinterpret_cast<const float4*>(d.in + first + j), l = *reinterpret_cast<const float4*>(d.in_lo + first + j);
+    f[j] = ex2((hi - h.x) + (lo - l.x)); f[j + 1] = ex2((hi - h.y) + (lo - l.y));
+    f[j + 2] = ex2((hi - h.z) + (lo - l.z)); f[j + 3] = ex2((hi - h.w) + (lo - l.w));
+  }
+}
+
+// Stretches of the units of a call.
+struct Cut {
+  int n_units, parts, per;      // parts of `per` chunks
+};
+struct Stretch { int unit, part, n, h, len, NT, lo, hi; };
+__device__ __forceinline__ Stretch stretch_of(const Tokens& t, const Cut& cut) {
+  Stretch x;
+  x.unit = blockIdx.x % cut.n_units; x.part = blockIdx.x / cut.n_units;
+  x.n = x.unit / t.H; x.h = x.unit % t.H;
+  x.len = t.length(x.n);
+  x.NT = (x.len + CT - 1) / CT;
+  x.lo = min(x.part * cut.per, x.NT);
+  x.hi = min(x.lo + cut.per, x.NT);
+  return x;
+}
+
+// rows n .. 127 of a chunk's token tile (they belong to the next sequence of a packed batch) as zeros
+__device__ __forceinline__ void zero_rows(unsigned char* tile, int n) {
+  for (int i = n * 8 + threadIdx.x; i < CT * 8; i += blockDim.x) *reinterpret_cast<uint4*>(tile + 16 * i) = make_uint4(0, 0, 0, 0);
+}
+
+Cut cut_units(int n_seq, int max_len, int H, bool backward);
+// the states (or their gradients) that the stretches start from, from what each adds; defined beside the forward
+int launch_chain(float* part_states, const float* part_decay, const float* first, int n_first, const Tokens& t, const Cut& cut, bool reverse,
+                 cudaStream_t st);
+
+// what every stretch adds to the gradient of the state before it (values d_o, keys r), walking backwards
+int launch_tc_add(const Args& a, const Cut& cut, const CUtensorMap& map_do, const CUtensorMap& map_r, float* part_states, float* part_decay, int* status,
+                  cudaStream_t st);
+
+}  // namespace la
+}  // namespace rwkvb200

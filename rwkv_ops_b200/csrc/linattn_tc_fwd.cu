@@ -1,0 +1,407 @@
+// Linear attention with a decay for each head, forward on tcgen05: bfloat16 tokens, head size 64 (linattn_tc.cuh).
+#include <algorithm>
+#include <type_traits>
+
+#include "linattn_tc.cuh"
+
+namespace rwkvb200 {
+namespace la {
+namespace {
+
+constexpr int NTHR = 256;
+
+struct FwdSmem {
+  unsigned char r[TOK_BYTES], k[TOK_BYTES], v[TOK_BYTES];      // k becomes the hi part of e^{Lc - L_j} k_j
+  unsigned char klo[TOK_BYTES];
+  unsigned char A[2][TOK_BYTES];      // A [token i][token j], two times 64 columns; the first half stages o afterwards
+  unsigned char S[TILE_BYTES];        // the state before the chunk, [v][k], rounded
+  Decays dec[2];
+  uint64_t bar_in, bar_1, bar_2;
+  uint32_t tmem_base;
+};
+constexpr uint32_t TM_S = 0, TM_O2 = 0, TM_U = 64, TM_O1 = 128, TM_COLS = 256;
+
+// One item: the chunks of a stretch in order, the state in registers (a row to the lower half lanes of a warp, 32 columns).  Per chunk two batches of
+// products with the threads' work between them:
+//   r k^T, r S^T            meanwhile the keys are scaled and split
+//   A v, v^T (scaled keys)  after A = (r k^T) * decays has been rounded and stored; then o and the next state
+// ADD: keys and values alone, from a zero state; what the stretch adds and its decay go to part_states / part_decay.  REV: the same for the
+// gradient of the state, from the last chunk to the first, with r for keys and d_o for values.
+// Two CTAs share an SM (113 KB each, 256 TMEM columns each), so that one's products and loads run under the other's arithmetic.
+template <bool PACKED, bool ADD, bool REV = false>
+__global__ void __launch_bounds__(NTHR, 2)
+la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int n_state, bf16* __restrict__ o, float* __restrict__ ht,
+                 float* __restrict__ states, float* __restrict__ part_states, float* __restrict__ part_decay,
+                 const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                 const __grid_constant__ CUtensorMap map_o, Tokens tok, Cut cut, int* status) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  FwdSmem& sm = *reinterpret_cast<FwdSmem*>(smem_raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wq = warp & 3, half = warp >> 2, row = 32 * wq + lane;      // the token whose row this thread reads, and which half of the columns
+  if (tid == 0) {
+    mbar_init(&sm.bar_in, 1); mbar_init(&sm.bar_1, 1); mbar_init(&sm.bar_2, 1);
+    fence_mbar_init();
+  }
+  if (tid == 32) tma_prefetch_maps(map_r, map_k, map_v, map_o);
+  if (warp == 0) tmem_alloc(&sm.tmem_base, TM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  earlier_kernels_done();
+  later_kernels_may_start();
+  const uint32_t tm = sm.tmem_base;
+  const Stretch x = stretch_of(tok, cut);
+  const int seq0 = PACKED ? __ldg(tok.start + x.n) : 0, brow = PACKED ? 0 : x.n;
+  const long long wb = tok.wbase(x.n, x.h);
+  auto rows_of = [&](int c) { return min(CT, x.len - c * CT); };
+  auto load_in = [&](int c) {      // one thread
+    const int t0 = seq0 + c * CT;
+    mbar_expect_tx(&sm.bar_in, (ADD ? 2 : 3) * TOK_BYTES);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      tma_load_4d(sm.k + q * TILE_BYTES, &map_k, &sm.bar_in, 0, t0 + 64 * q, x.h, brow);
+      if constexpr (!ADD) tma_load_4d(sm.r + q * TILE_BYTES, &map_r, &sm.bar_in, 0, t0 + 64 * q, x.h, brow);
+      tma_load_4d(sm.v + q * TILE_BYTES, &map_v, &sm.bar_in, 0, t0 + 64 * q, x.h, brow);
+    }
+  };
+  // the state: lanes 0 .. 15 hold row v = 16 wq + lane, columns 32 half .. + 31
+  const bool st_lane = lane < 16;
+  const int srow = 16 * wq + (lane & 15);
+  const long long sat = (long long)srow * 64 + 32 * half;
+  float S[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) S[j] = 0.f;
+  auto put_state = [&](float* to) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(to + sat + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+  };
+  bool ok = true;
+  float decay = 1.f;
+  const int n_chunks = x.hi - x.lo;
+  auto chunk = [&](int i) { return REV ? x.hi - 1 - i : x.lo + i; };      // the i-th
+  if (n_chunks > 0) {
+    if (warp == 0 && elect_one()) load_in(chunk(0));
+    RawW raw;
+    auto load_raw = [&](int i) {
+      if (i < n_chunks) raw = load_w(tok, w, wb, chunk(i) * CT, rows_of(chunk(i)));
+    };
+    if (warp == 4) {      // the decays are this warp's job: it has no block of A below the diagonal in its half
+      load_raw(0);
+      make_decays(sm.dec[0], raw, rows_of(chunk(0)), nullptr);
+      load_raw(1);
+    }
+    if constexpr (!ADD) {
+      if (st_lane) {
+        const float* from = x.part ? part_states + ((long long)x.unit * cut.parts + x.part) * 4096
+                            : h0   ? h0 + ((long long)(n_state == 1 ? 0 : x.n) * tok.H + x.h) * 4096 : nullptr;
+        if (from) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(from + sat + j));
+            S[j] = f.x; S[j + 1] = f.y; S[j + 2] = f.z; S[j + 3] = f.w;
+          }
+        }
+        if (states) put_state(states + ((long long)x.unit * tok.NT + x.lo) * 4096);
+        tile_store_row32(sm.S, srow, 32 * half, S);
+      }
+      // A above the diagonal of blocks: never written again
+      for (int e = tid; e < CT * 8; e += NTHR) *reinterpret_cast<uint4*>(sm.A[1] + 16 * e) = make_uint4(0, 0, 0, 0);
+    }
+    fence_async_smem();
+    __syncthreads();
+    for (int i = 0; i < n_chunks; ++i) {
+      const int c = chunk(i);
+      const uint32_t ph = i & 1;
+      const Decays& d = sm.dec[ph];
+      const int n = rows_of(c);
+      ok = mbar_wait(&sm.bar_in, ph, status, 501) && ok;
+      if (PACKED && n < CT) {
+        zero_rows(sm.k, n);
+        zero_rows(sm.v, n);
+        fence_async_smem();
+        __syncthreads();
+      }
+      if constexpr (!ADD) {
+        if (warp == 0 && elect_one()) {
+          bulk_wait_read();      // o of the chunk before has left its place in A
+          tc_fence_after();
+          umma_tile<128, 128, 0, 0>(tmem_addr(tm, 0, TM_S), smem_u32(sm.r), smem_u32(sm.k), false);
+          umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_O1), smem_u32(sm.r), smem_u32(sm.S), false);
+          umma_commit(&sm.bar_1);
+        }
+      }
+      // scaled keys, 32 columns of a token; the hi part waits until the products have read the keys as they are
+      uint4 hi[4];
+      {
+        const float f = REV ? d.start[row] : d.end[row];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t off = (row >> 6) * TILE_BYTES + tile_chunk_off(row & 63, 4 * half + q);
+          const uint4 u = *reinterpret_cast<const uint4*>(sm.k + off);
+          uint4 lo;
+          const uint32_t in[4] = {u.x, u.y, u.z, u.w};
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float a = bf16_lo(in[e]) * f, b = bf16_hi(in[e]) * f;
+            h[e] = pack_bf16(a, b);
+            l[e] = pack_bf16(a - bf16_lo(h[e]), b - bf16_hi(h[e]));
+          }
+          hi[q] = make_uint4(h[0], h[1], h[2], h[3]);
+          lo = make_uint4(l[0], l[1], l[2], l[3]);
+          *reinterpret_cast<uint4*>(sm.klo + off) = lo;
+        }
+      }
+      if constexpr (!ADD) {
+        ok = mbar_wait(&sm.bar_1, ph, status, 502) && ok;
+        tc_fence_after();
+      } else {
+        __syncwarp();
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<uint4*>(sm.k + (row >> 6) * TILE_BYTES + tile_chunk_off(row & 63, 4 * half + q)) = hi[q];
+      if constexpr (!ADD) {
+        // A: blocks of 32 x 32 on and below the diagonal (warp: rows 32 wq .., columns 64 half ..)
+        unsigned char* At = sm.A[half] + (row >> 6) * TILE_BYTES;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int J = 2 * half + b;
+          float p[32];
+          if (J <= wq) {
+            uint32_t s[32];
+            tmem_ld32(tmem_addr(tm, 32 * wq, TM_S + 32 * J), s);
+            if (J < wq) {
+              const float f = d.row[row];
+              const float* col = d.col[wq - 1] + 32 * J;
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                const float4 g = *reinterpret_cast<const float4*>(col + j);
+                p[j] = __uint_as_float(s[j]) * (f * g.x); p[j + 1] = __uint_as_float(s[j + 1]) * (f * g.y);
+                p[j + 2] = __uint_as_float(s[j + 2]) * (f * g.z); p[j + 3] = __uint_as_float(s[j + 3]) * (f * g.w);
+              }
+            } else {
+              diagonal_factors(d, row, 32 * J, p);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) p[j] = j <= lane ? __uint_as_float(s[j]) * p[j] : 0.f;
+            }
+            tile_store_row32(At, row & 63, 32 * b, p);
+          } else if (J == 1) {      // (wq == 0: the staged o was here)
+#pragma unroll
+            for (int j = 0; j < 32; ++j) p[j] = 0.f;
+            tile_store_row32(At, row & 63, 32 * b, p);
+          }
+        }
+      }
+      if (warp == 4 && i + 1 < n_chunks) {
+        make_decays(sm.dec[ph ^ 1], raw, rows_of(chunk(i + 1)), nullptr);
+        load_raw(i + 2);
+      }
+      fence_async_smem();
+      tc_fence_before();
+      __syncthreads();
+      if (warp == 0 && elect_one()) {
+        tc_fence_after();
+        if constexpr (!ADD) {
+          umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_O2), smem_u32(sm.A[0]), smem_u32(sm.v), false);
+          umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_O2), smem_u32(sm.A[1]), smem_u32(sm.v) + TILE_BYTES, true);
+        }
+        umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.k), false);
+        umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.klo), true);
+        umma_commit(&sm.bar_2);
+      }
+      ok = mbar_wait(&sm.bar_2, ph, status, 503) && ok;
+      tc_fence_after();
+      if (i + 1 < n_chunks && warp == 0 && elect_one()) load_in(chunk(i + 1));
+      const float all = d.all;
+      {
+        uint32_t u[32];
+        tmem_ld32(tmem_addr(tm, 32 * wq, TM_U + 32 * half), u);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 32; ++j) S[j] = fmaf(all, S[j], __uint_as_float(u[j]));
+      }
+      if constexpr (ADD) {
+        decay *= all;
+      } else {
+        if (st_lane) {
+          tile_store_row32(sm.S, srow, 32 * half, S);
+          if (states && c + 1 < x.hi) put_state(states + ((long long)x.unit * tok.NT + c + 1) * 4096);
+        }
+        uint32_t a[32], b[32];
+        tmem_ld32(tmem_addr(tm, 32 * wq, TM_O1 + 32 * half), a);
+        tmem_ld32(tmem_addr(tm, 32 * wq, TM_O2 + 32 * half), b);
+        tmem_ld_wait();
+        const float f = d.start[row];
+        float y[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) y[j] = fmaf(f, __uint_as_float(a[j]), __uint_as_float(b[j]));
+        if (!o) {                    // (the states alone)
+        } else if (PACKED && n < CT) {      // the rows behind belong to the next sequence
+          if (row < n) {
+            bf16* to = o + tok.base(x.n, x.h) + (long long)(c * CT + row) * tok.st + 32 * half;
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              *reinterpret_cast<uint4*>(to + j) = make_uint4(pack_bf16(y[j], y[j + 1]), pack_bf16(y[j + 2], y[j + 3]),
+                                                             pack_bf16(y[j + 4], y[j + 5]), pack_bf16(y[j + 6], y[j + 7]));
+          }
+        } else {
+          tile_store_row32(sm.A[0] + (row >> 6) * TILE_BYTES, row & 63, 32 * half, y);
+        }
+      }
+      fence_async_smem();
+      tc_fence_before();
+      if (!__syncthreads_and(ok)) break;
+      if (!ADD && o && !(PACKED && n < CT) && warp == 0 && elect_one()) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q)      // (rows past the end of the batch are clipped)
+          if (64 * q < n) tma_store_4d(&map_o, sm.A[0] + q * TILE_BYTES, 0, seq0 + c * CT + 64 * q, x.h, brow);
+        bulk_commit();
+      }
+    }
+  } else if (!ADD && st_lane) {      // no chunk: a sequence without tokens hands its state on
+    if (x.part == 0 && h0) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j) S[j] = h0[((long long)(n_state == 1 ? 0 : x.n) * tok.H + x.h) * 4096 + sat + j];
+    }
+  }
+  if constexpr (ADD) {
+    if (st_lane) put_state(part_states + ((long long)x.unit * cut.parts + x.part) * 4096);
+    if (tid == 0) part_decay[(long long)x.unit * cut.parts + x.part] = decay;
+  } else {
+    if (st_lane && ht && (x.NT == 0 ? x.part == 0 : x.lo < x.hi && x.hi == x.NT)) put_state(ht + (long long)x.unit * 4096);
+  }
+  if (warp == 0 && elect_one()) bulk_wait_all();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tm, TM_COLS);
+}
+
+// part_states[unit][p] becomes the state that stretch p starts from (reverse: the gradient of the state that it ends with), from what each stretch adds.
+__global__ void __launch_bounds__(256) la_chain_kernel(float* __restrict__ part, const float* __restrict__ decay, const float* __restrict__ first,
+                                                       int n_first, int H, int n_units, int parts, int reverse) {
+  earlier_kernels_done();
+  later_kernels_may_start();
+  const int i = blockIdx.x * 256 + threadIdx.x, unit = i >> 10, e = 4 * (i & 1023);
+  if (unit >= n_units) return;
+  float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (first) S = *reinterpret_cast<const float4*>(first + (n_first == 1 ? (long long)(unit % H) : (long long)unit) * 4096 + e);
+  float* p0 = part + (long long)unit * parts * 4096 + e;
+  constexpr int AHEAD = 8;
+  for (int q0 = 0; q0 < parts; q0 += AHEAD) {
+    float4 add[AHEAD];
+    float f[AHEAD];
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      if (q0 + q < parts) {
+        const int p = reverse ? parts - 1 - q0 - q : q0 + q;
+        add[q] = *reinterpret_cast<const float4*>(p0 + (long long)p * 4096);
+        f[q] = decay[(long long)unit * parts + p];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      if (q0 + q < parts) {
+        const int p = reverse ? parts - 1 - q0 - q : q0 + q;
+        *reinterpret_cast<float4*>(p0 + (long long)p * 4096) = S;
+        S.x = fmaf(f[q], S.x, add[q].x); S.y = fmaf(f[q], S.y, add[q].y);
+        S.z = fmaf(f[q], S.z, add[q].z); S.w = fmaf(f[q], S.w, add[q].w);
+      }
+    }
+  }
+}
+
+template <bool PACKED>
+int fwd(const Args& a, cudaStream_t st) {
+  const Tokens& t = a.tok;
+  DeviceFacts f;
+  if (int e = device_facts(&f)) return e;
+  constexpr int smem = (int)sizeof(FwdSmem);
+  static_assert(smem <= 115712, "two CTAs of 113 KB each share an SM");
+  if (int e = need_aligned_smem<la_tc_fwd_kernel<PACKED, false>>(f)) return e;
+  if (int e = need_aligned_smem<la_tc_fwd_kernel<PACKED, true>>(f)) return e;
+  if (int e = allow_smem<la_tc_fwd_kernel<PACKED, false>>(f, smem)) return e;
+  if (int e = allow_smem<la_tc_fwd_kernel<PACKED, true>>(f, smem)) return e;
+  const int B = t.start ? 1 : t.n_seq, T = t.start ? (int)a.w_rows : t.T, head_first = t.st == 64 && t.H > 1;
+  CUtensorMap mr, mk, mv, mo;
+  const void* r = a.r ? a.r : a.k;      // (the states alone: r is not loaded, o not stored)
+  void* o = a.o ? a.o : const_cast<void*>(a.k);
+  if (int e = make_token_tensor_map(&mr, r, B, T, t.H, head_first)) return e;
+  if (int e = make_token_tensor_map(&mk, a.k, B, T, t.H, head_first)) return e;
+  if (int e = make_token_tensor_map(&mv, a.v, B, T, t.H, head_first)) return e;
+  if (int e = make_token_tensor_map(&mo, o, B, T, t.H, head_first)) return e;
+  const Cut cut = cut_units(t.n_seq, t.T, t.H, false);
+  float* part_states = static_cast<float*>(a.scratch);
+  float* part_decay = part_states + (size_t)cut.n_units * cut.parts * 4096;
+  if (cut.parts > 1) {
+    {
+      ProfScope prof("linattn_tc_add_kernel", st);
+      if (int e = launch(la_tc_fwd_kernel<PACKED, true>, cut.n_units * cut.parts, NTHR, smem, st, 1, a.w, a.h0, a.n_state, (bf16*)a.o, a.ht, a.states,
+                         part_states, part_decay, mr, mk, mv, mo, t, cut, f.status)) return e;
+    }
+    if (int e = launch_chain(part_states, part_decay, a.h0, a.n_state, t, cut, false, st)) return e;
+  }
+  ProfScope prof("linattn_tc_fwd_kernel", st);
+  return launch(la_tc_fwd_kernel<PACKED, false>, cut.n_units * cut.parts, NTHR, smem, st, 1, a.w, a.h0, a.n_state, (bf16*)a.o, a.ht, a.states, part_states,
+                part_decay, mr, mk, mv, mo, t, cut, f.status);
+}
+
+}  // namespace
+
+int launch_tc_add(const Args& a, const Cut& cut, const CUtensorMap& map_do, const CUtensorMap& map_r, float* part_states, float* part_decay, int* status,
+                  cudaStream_t st) {
+  ProfScope prof("linattn_tc_add_kernel", st);
+  constexpr int smem = (int)sizeof(FwdSmem);
+  DeviceFacts f;
+  if (int e = device_facts(&f)) return e;
+  const auto go = [&](auto packed) {
+    constexpr bool PACKED = decltype(packed)::value;
+    if (int e = need_aligned_smem<la_tc_fwd_kernel<PACKED, true, true>>(f)) return e;
+    if (int e = allow_smem<la_tc_fwd_kernel<PACKED, true, true>>(f, smem)) return e;
+    return launch(la_tc_fwd_kernel<PACKED, true, true>, cut.n_units * cut.parts, NTHR, smem, st, 1, a.w, (const float*)nullptr, 0, (bf16*)nullptr,
+                  (float*)nullptr, (float*)nullptr, part_states, part_decay, map_r, map_r, map_do, map_r, a.tok, cut, status);
+  };
+  return a.tok.start ? go(std::true_type()) : go(std::false_type());
+}
+
+int launch_chain(float* part_states, const float* part_decay, const float* first, int n_first, const Tokens& t, const Cut& cut, bool reverse,
+                 cudaStream_t st) {
+  ProfScope prof("linattn_chain_kernel", st);
+  return launch(la_chain_kernel, cut.n_units * 4, 256, 0, st, 1, part_states, part_decay, first, n_first, t.H, cut.n_units, cut.parts, (int)reverse);
+}
+
+// How many stretches: as many as the device holds CTAs, where the walk over the chunks that they save is longer than the pass over keys and values and the
+// two launches that they cost (about three chunks' time).
+Cut cut_units(int n_seq, int max_len, int H, bool backward) {
+  const int SLOTS = backward ? 148 : 2 * 148;      // CTAs that a B200 holds
+  const int NT = (max_len + CT - 1) / CT;
+  Cut c;
+  c.n_units = n_seq * H;
+  c.parts = std::max(1, std::min(NT, SLOTS / c.n_units));
+  c.per = (NT + c.parts - 1) / c.parts;
+  if (c.parts > 1 && NT - 1.6 * c.per < 3) c.per = NT;
+  c.parts = (NT + c.per - 1) / c.per;
+  return c;
+}
+
+size_t tc_states_bytes(int n_seq, int max_len, int H, bool keep) {
+  return keep ? (size_t)n_seq * H * ((max_len + CT - 1) / CT) * 4096 * 4 : 0;
+}
+
+size_t tc_scratch_bytes(int n_seq, int max_len, int H, bool w_per_head, bool backward) {
+  const Cut c = cut_units(n_seq, max_len, H, backward);
+  size_t n = c.parts > 1 ? (size_t)c.n_units * c.parts * (4096 + 1) * 4 : 0;
+  if (backward && w_per_head) n = (n + 255) / 256 * 256 + ((size_t)n_seq * c.parts * H * 4 + 255) / 256 * 256 + (size_t)DW_PARTS * H * 8;
+  return n;
+}
+
+int launch_tc_fwd(const Args& a, cudaStream_t st) {
+  Args b = a;
+  b.tok.NT = (a.tok.T + CT - 1) / CT;
+  return a.tok.start ? fwd<true>(b, st) : fwd<false>(b, st);
+}
+
+}  // namespace la
+}  // namespace rwkvb200

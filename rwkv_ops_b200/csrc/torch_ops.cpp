@@ -7,7 +7,9 @@
 // Every public function of the Python modules is one operator here:
 //   generalized_delta_rule, rwkv7_varlen, rwkv7_fused, wkv6, wkv6_varlen   composite: checks, conversions, then
 //   rwkv7_fwd / _bwd, rwkv7_fwd_varlen / _bwd_varlen, ...                  one C-ABI call each (CUDA), autograd
-//   rwkv7_decode_step                                                      one C-ABI call, in place on the state
+//   linear_attention                                                       the same over linattn_fwd / _bwd
+//   rwkv7_decode_step, linattn_step, reorder_states                        one C-ABI call, in place on the state
+//   beam_select                                                            one C-ABI call
 // The composite operators raise on every argument the Python layer documents as invalid; the Python layer then
 // repeats its own checks to raise the documented exception type.  The shape functions of the CUDA operators
 // (for tracing without a device) are registered from Python (_ops.py).
@@ -752,12 +754,221 @@ std::tuple<Tensor, Tensor> wkv6_varlen(const Tensor& r, const Tensor& k, const T
 }
 
 // ---------------------------------------------------------------------------------------------
+// linear attention with a decay for each head, dense or packed (seq_start, seq_len, max_len)
+// ---------------------------------------------------------------------------------------------
+typedef std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> Five;
+struct LaDims { int n_seq, max_len, total, H, D; };
+LaDims linattn_dims(const Tensor& r, const OptTensor& seq_start, int64_t max_len, bool head_first) {
+  const Dims d = dims_of(r, head_first);
+  if (has(seq_start)) return {(int)seq_start->numel(), (int)max_len, d.T, d.H, d.K};
+  return {d.B, d.T, 0, d.H, d.K};
+}
+// the states between chunks into `states` (undefined: none are left), and o, ht where they are defined
+void linattn_forward(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const OptTensor& seq_start, const OptTensor& seq_len,
+                     const LaDims& d, const OptTensor& h0, bool head_first, const Tensor& o, const Tensor& ht, const Tensor& kept) {
+  const int code = dtype_code(r.scalar_type()), per_head = w.dim() == 1;
+  const size_t ns = rwkvb200_linattn_states_bytes(d.n_seq, d.max_len, d.H, d.D, code, kept.defined());
+  const size_t nw = rwkvb200_linattn_workspace_bytes(d.n_seq, d.max_len, d.total, d.H, d.D, code, per_head, 0);
+  const Tensor states = kept.defined() ? kept : ns ? bytes(ns, r) : Tensor(), ws = nw ? bytes(nw, r) : Tensor();
+  check(rwkvb200_linattn_fwd(ptr(r), fptr(w), per_head, ptr(k), ptr(v), fptr(h0), n_state_of(h0), ptr(o), fptr(ht), fptr(states), ns, ptr(ws), nw,
+                             iptr(seq_start), iptr(seq_len), d.n_seq, d.max_len, d.total, d.H, d.D, code, head_first, stream_of(r)),
+        "linattn_fwd");
+}
+
+Three linattn_fwd(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const OptTensor& seq_start, const OptTensor& seq_len,
+                  int64_t max_len, const OptTensor& h0, bool head_first, bool keep) {
+  const c10::cuda::CUDAGuard guard(r.device());
+  const LaDims d = linattn_dims(r, seq_start, max_len, head_first);
+  Tensor o = fresh_like(r), ht = fresh({d.n_seq, d.H, d.D, d.D}, at::kFloat, r), kept;
+  if (keep) kept = bytes(rwkvb200_linattn_states_bytes(d.n_seq, d.max_len, d.H, d.D, dtype_code(r.scalar_type()), 1), r);
+  linattn_forward(r, w, k, v, seq_start, seq_len, d, h0, head_first, o, ht, kept);
+  return {o, ht, keep ? kept : bytes(0, r)};
+}
+
+// `kept` (may be empty: they are computed again): the states that a forward with keep left; they are not changed.
+Five linattn_bwd(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const OptTensor& seq_start, const OptTensor& seq_len,
+                 int64_t max_len, const OptTensor& h0, const Tensor& d_o, const OptTensor& d_ht, const Tensor& kept, bool head_first) {
+  const c10::cuda::CUDAGuard guard(r.device());
+  const LaDims d = linattn_dims(r, seq_start, max_len, head_first);
+  const int code = dtype_code(r.scalar_type()), per_head = w.dim() == 1;
+  Tensor dr = fresh_like(r), dw = fresh_like(w), dk = fresh_like(r), dv = fresh_like(r), dh0 = fresh({d.n_seq, d.H, d.D, d.D}, at::kFloat, r);
+  const size_t ns = rwkvb200_linattn_states_bytes(d.n_seq, d.max_len, d.H, d.D, code, 1);
+  const size_t nw = rwkvb200_linattn_workspace_bytes(d.n_seq, d.max_len, d.total, d.H, d.D, code, per_head, 1);
+  Tensor states = kept;
+  if ((size_t)kept.numel() < ns) {
+    states = bytes(ns, r);
+    linattn_forward(r, w, k, v, seq_start, seq_len, d, h0, head_first, Tensor(), Tensor(), states);
+  }
+  const Tensor ws = nw ? bytes(nw, r) : Tensor();
+  check(rwkvb200_linattn_bwd(ptr(r), fptr(w), per_head, ptr(k), ptr(v), ptr(d_o), fptr(d_ht), fptr(states), ns, ptr(dr), fptr(dw), ptr(dk), ptr(dv),
+                             fptr(dh0), ptr(ws), nw, iptr(seq_start), iptr(seq_len), d.n_seq, d.max_len, d.total, d.H, d.D, code, head_first,
+                             stream_of(r)), "linattn_bwd");
+  return {dr, dw, dk, dv, dh0};
+}
+
+struct LinattnFn : torch::autograd::Function<LinattnFn> {
+  static Vars forward(Ctx* ctx, const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const OptTensor& seq_start,
+                      const OptTensor& seq_len, int64_t max_len, const OptTensor& h0, bool head_first, bool keep) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [o, ht, kept] = RWKV_OP(linattn_fwd, "linattn_fwd", r, w, k, v, seq_start, seq_len, max_len, h0, head_first, keep);
+    ctx->save_for_backward({r, w, k, v, has(seq_start) ? *seq_start : Tensor(), has(seq_len) ? *seq_len : Tensor(), has(h0) ? *h0 : Tensor(), kept});
+    ctx->set_materialize_grads(false);
+    ctx->mark_non_differentiable({kept});
+    ctx->saved_data["max_len"] = max_len;
+    ctx->saved_data["head_first"] = head_first;
+    return {o, ht, kept};
+  }
+  static Vars backward(Ctx* ctx, Vars g) {
+    const Vars s = ctx->get_saved_variables();
+    const auto opt = [](const Tensor& x) { return x.defined() ? OptTensor(x) : std::nullopt; };
+    const OptTensor h0 = opt(s[6]);
+    auto [dr, dw, dk, dv, dh0] =
+        RWKV_OP(linattn_bwd, "linattn_bwd", s[0], s[1], s[2], s[3], opt(s[4]), opt(s[5]), ctx->saved_data["max_len"].toInt(), h0,
+                token_grad(g[0], s[0]), final_state_grad(g[1]), s[7], ctx->saved_data["head_first"].toBool());
+    const size_t at = s[4].defined() ? 6 : 4;      // (inputs that are not there are not counted)
+    const Tensor ds = has(h0) && ctx->needs_input_grad(at) ? state_grad(dh0, h0) : Tensor();
+    return {dr, dw, dk, dv, Tensor(), Tensor(), Tensor(), ds, Tensor(), Tensor()};
+  }
+};
+
+Three linattn_fwd_autograd(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const OptTensor& seq_start, const OptTensor& seq_len,
+                           int64_t max_len, const OptTensor& h0, bool head_first, bool keep) {
+  if (any_requires_grad({&r, &w, &k, &v}, h0)) {
+    Vars out = LinattnFn::apply(r, w, k, v, seq_start, seq_len, max_len, h0, head_first, keep);
+    return {out[0], out[1], out[2]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return RWKV_OP(linattn_fwd, "linattn_fwd", r, w, k, v, seq_start, seq_len, max_len, h0, head_first, keep);
+}
+
+std::tuple<Tensor, Tensor> linear_attention(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const OptTensor& seq_start,
+                                            const OptTensor& seq_len, int64_t max_len, const OptTensor& initial_state, bool head_first) {
+  check_tokens(r, {&k, &v}, 4);
+  const SymDims d = sym_dims_of(r, head_first);
+  TORCH_CHECK_VALUE(d.K == 64 || d.K == 128, "head size must be 64 or 128, got ", d.K);
+  TORCH_CHECK_VALUE(w.is_cuda() && w.device() == r.device() &&
+                        (w.dim() == 1 ? w.sym_size(0) == d.H
+                                      : w.dim() == 3 && w.sym_size(0) == d.B && w.sym_size(1) == r.sym_size(1) && w.sym_size(2) == r.sym_size(2)),
+                    "w must be [", d.H, "] or one number per token and head, got ", w.sym_sizes());
+  const bool packed = has(seq_start);
+  TORCH_CHECK_VALUE(!packed || d.B == 1, "expected packed token tensors [1, total_len, H, D], got ", r.sym_sizes());
+  const SymInt n_seq = packed ? seq_start->sym_numel() : d.B;
+  check_state(initial_state, r, n_seq, d.H, d.K);
+  const at::ScalarType t = compute_dtype(r.scalar_type());
+  const Tensor r_ = dense(r, t), w_ = dense(w, at::kFloat), k_ = dense(k, t), v_ = dense(v, t);
+  const OptTensor h0 = dense_state(initial_state);
+  bool keep = false;
+  if (any_requires_grad({&r_, &w_, &k_, &v_}, h0)) {
+    const auto limit = (int64_t)std::min<size_t>(keep_limit_bytes(r.device().index()), std::numeric_limits<int64_t>::max());
+    const SymInt len = packed ? SymInt(max_len) : d.T;
+    // (rwkvb200_linattn_states_bytes, of sizes that may be symbols)
+    const SymInt chunks = d.K == HEAD && t == at::kBFloat16 ? (len + 127) / 128 : (len + 63) / 64 + 1;
+    keep = TORCH_STATICALLY_KNOWN_TRUE((n_seq * d.H * chunks * d.K * d.K * 4).sym_le(limit));
+  }
+  auto [o, ht, kept] = RWKV_OP(linattn_fwd, "linattn_fwd", r_, w_, k_, v_, seq_start, seq_len, max_len, h0, head_first, keep);
+  return {o.to(r.scalar_type()), ht};
+}
+
+// ---------------------------------------------------------------------------------------------
+// states kept on the device: one token of linear attention in place, and reordering by beam
+// ---------------------------------------------------------------------------------------------
+// parents as the kernels take them: [groups, beams], whole numbers
+Tensor beam_parents(const Tensor& parents, const Tensor& state) {
+  TORCH_CHECK_VALUE(parents.dim() == 2 && parents.device() == state.device() && !parents.is_floating_point() && !parents.is_complex() &&
+                        parents.numel() == state.size(0) && parents.size(1) >= 1 && parents.size(1) <= 32,
+                    "parents must be [groups, beams], at most 32 beams and ", state.size(0), " in all, got ", parents.sizes());
+  return parents.to(at::kLong).contiguous();
+}
+void changed(const Tensor& state) {
+  if (!state.is_inference()) state.unsafeGetTensorImpl()->bump_version();
+}
+
+Tensor linattn_step(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, Tensor state, const OptTensor& parents) {
+  check_tokens(r, {&k, &v}, (int)r.dim());
+  const int64_t B = state.size(0), H = state.size(1), D = state.size(3);
+  TORCH_CHECK_VALUE((r.dim() == 3 || (r.dim() == 4 && r.size(1) == 1)) && r.size(0) == B && r.size(r.dim() - 2) == H &&
+                        r.size(-1) == D && state.is_contiguous() && state.device() == r.device(),
+                    "expected token tensors [", B, ", 1, ", H, ", ", D, "] or [", B, ", ", H, ", ", D, "], got ", r.sizes());
+  TORCH_CHECK_VALUE(w.device() == r.device() && (w.dim() == 1 ? w.size(0) == H : w.sizes() == r.sizes().slice(0, r.dim() - 1)),
+                    "w must be [", H, "] or one number per token and head, got ", w.sizes());
+  const c10::cuda::CUDAGuard guard(r.device());
+  const at::ScalarType t = compute_dtype(r.scalar_type());
+  const Tensor r_ = dense(r, t), w_ = dense(w, at::kFloat), k_ = dense(k, t), v_ = dense(v, t);
+  const Tensor p = has(parents) ? beam_parents(*parents, state) : Tensor();
+  const int beams = p.defined() ? (int)p.size(1) : 1;
+  Tensor o = fresh_like(r_);
+  check(rwkvb200_linattn_step(ptr(r_), fptr(w_), w_.dim() == 1, ptr(k_), ptr(v_), ptr(state), dtype_code(state.scalar_type()), ptr(o),
+                              p.defined() ? p.data_ptr<int64_t>() : nullptr, (int)(B / beams), beams, (int)H, (int)D, dtype_code(t), stream_of(r)),
+        "linattn_step");
+  return o.to(r.scalar_type());
+}
+Tensor linattn_step_autograd(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, Tensor state, const OptTensor& parents) {
+  Tensor o;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    o = RWKV_OP(linattn_step, "linattn_step", r, w, k, v, state, parents);
+  }
+  changed(state);
+  return o;
+}
+
+void reorder_states(Tensor state, const Tensor& parents) {
+  TORCH_CHECK_VALUE(state.is_cuda() && state.dim() >= 1 && state.is_contiguous() && state.size(0) > 0 && state.numel() > 0,
+                    "expected a contiguous CUDA tensor of states, got ", state.sizes());
+  const int64_t row = state.numel() / state.size(0) * (int64_t)state.element_size();
+  TORCH_CHECK_VALUE(row % 16 == 0, "a state must be a multiple of 16 bytes, got ", row);
+  const Tensor p = beam_parents(parents, state);
+  const c10::cuda::CUDAGuard guard(state.device());
+  check(rwkvb200_reorder_states(ptr(state), p.data_ptr<int64_t>(), (int)p.size(0), (int)p.size(1), (size_t)row, stream_of(state)), "reorder_states");
+}
+void reorder_states_autograd(Tensor state, const Tensor& parents) {
+  TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && state.requires_grad()), "states that are reordered in place cannot require gradients");
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    RWKV_OP(reorder_states, "reorder_states", state, parents);
+  }
+  changed(state);
+}
+
+// ---------------------------------------------------------------------------------------------
+// beam search
+// ---------------------------------------------------------------------------------------------
+std::tuple<Tensor, Tensor, Tensor, Tensor> beam_select(const Tensor& logits, const Tensor& scores, const OptTensor& finished, int64_t eos) {
+  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 3 && logits.numel() > 0, "expected logits [groups, beams, vocabulary], got ", logits.sizes());
+  const int64_t G = logits.size(0), W = logits.size(1), V = logits.size(2);
+  TORCH_CHECK_VALUE(scores.device() == logits.device() && scores.sizes() == logits.sizes().slice(0, 2), "scores must be [", G, ", ", W, "], got ",
+                    scores.sizes());
+  TORCH_CHECK_VALUE(W <= 32 && V <= (1 << 30) && G <= std::numeric_limits<int>::max(), "at most 32 beams and 2^30 tokens, got ", logits.sizes());
+  TORCH_CHECK_VALUE(eos < V && (eos >= 0 || !has(finished)), "eos must be a token, got ", eos);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  Tensor x = logits.to(compute_dtype(logits.scalar_type()));
+  if (x.stride(2) != 1 || x.stride(0) < 0 || x.stride(1) < 0) x = x.contiguous();
+  const Tensor s = dense(scores, at::kFloat);
+  Tensor f;
+  if (has(finished)) {
+    TORCH_CHECK_VALUE(finished->device() == logits.device() && finished->sizes() == scores.sizes(), "finished must be like scores, got ", finished->sizes());
+    f = finished->to(at::kBool).contiguous();
+  }
+  Tensor best = fresh({G, W}, at::kFloat, x), parents = fresh({G, W}, at::kLong, x), tokens = fresh({G, W}, at::kLong, x),
+         done = fresh(eos >= 0 ? at::IntArrayRef{G, W} : at::IntArrayRef{0}, at::kBool, x);
+  check(rwkvb200_beam_select(ptr(x), dtype_code(x.scalar_type()), x.stride(0), x.stride(1), fptr(s), static_cast<const uint8_t*>(ptr(f)), eos, fptr(best),
+                             parents.data_ptr<int64_t>(), tokens.data_ptr<int64_t>(), eos >= 0 ? static_cast<uint8_t*>(ptr(done)) : nullptr, (int)G, (int)W,
+                             (int)V, stream_of(x)), "beam_select");
+  return {best, parents, tokens, done};
+}
+// a selection is not differentiated
+std::tuple<Tensor, Tensor, Tensor, Tensor> beam_select_autograd(const Tensor& logits, const Tensor& scores, const OptTensor& finished, int64_t eos) {
+  at::AutoDispatchBelowADInplaceOrView below;
+  return RWKV_OP(beam_select, "beam_select", logits, scores, finished, eos);
+}
+
+// ---------------------------------------------------------------------------------------------
 // the backward operators under autograd: a gradient can be asked for with create_graph, but differentiating it again is an
 // error, not a silent zero
 // ---------------------------------------------------------------------------------------------
 constexpr char RWKV7_BWD[] = "rwkv_ops_b200::rwkv7_bwd", RWKV7_BWD_VARLEN[] = "rwkv_ops_b200::rwkv7_bwd_varlen",
                RWKV7_FUSED_BWD[] = "rwkv_ops_b200::rwkv7_fused_bwd", WKV6_BWD[] = "rwkv_ops_b200::wkv6_bwd",
-               WKV6_BWD_VARLEN[] = "rwkv_ops_b200::wkv6_bwd_varlen";
+               WKV6_BWD_VARLEN[] = "rwkv_ops_b200::wkv6_bwd_varlen", LINATTN_BWD[] = "rwkv_ops_b200::linattn_bwd";
 
 void differentiable_inputs(Vars& to, const Tensor& x) { if (x.defined() && x.requires_grad()) to.push_back(x); }
 void differentiable_inputs(Vars& to, const OptTensor& x) { if (has(x)) differentiable_inputs(to, *x); }
@@ -802,6 +1013,13 @@ TORCH_LIBRARY(rwkv_ops_b200, m) {
   m.def("rwkv7_fused(" FUSED_SIX ", Tensor? initial_state) -> (Tensor, Tensor)", rwkv7_fused);
   m.def("rwkv7_fused_fwd(" FUSED_SIX ", Tensor? h0, bool keep) -> (Tensor, Tensor, Tensor)");
   m.def("rwkv7_fused_bwd(" FUSED_SIX ", Tensor? h0, Tensor d_o, Tensor? d_ht, Tensor kept) -> " OUT7);
+#define LINATTN "Tensor r, Tensor w, Tensor k, Tensor v, Tensor? seq_start, Tensor? seq_len, int max_len"
+  m.def("linear_attention(" LINATTN ", Tensor? initial_state, bool head_first) -> (Tensor, Tensor)", linear_attention);
+  m.def("linattn_fwd(" LINATTN ", Tensor? h0, bool head_first, bool keep) -> (Tensor, Tensor, Tensor)");
+  m.def("linattn_bwd(" LINATTN ", Tensor? h0, Tensor d_o, Tensor? d_ht, Tensor kept, bool head_first) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("linattn_step(Tensor r, Tensor w, Tensor k, Tensor v, Tensor(a!) state, Tensor? parents) -> Tensor");
+  m.def("reorder_states(Tensor(a!) state, Tensor parents) -> ()");
+  m.def("beam_select(Tensor logits, Tensor scores, Tensor? finished, int eos) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("wkv6(" FIVE ", int head_size, Tensor? init_state, Tensor? state_map, bool with_state) -> (Tensor, Tensor)", wkv6);
   m.def("wkv6_fwd(" FIVE ", Tensor? s0, Tensor? state_map, int algo, bool keep) -> (Tensor, Tensor, Tensor)");
   m.def("wkv6_bwd(" FIVE ", Tensor? s0, Tensor? state_map, Tensor d_y, Tensor? d_sT, Tensor kept, int algo) -> " OUT6);
@@ -822,6 +1040,11 @@ TORCH_LIBRARY_IMPL(rwkv_ops_b200, CUDA, m) {
   m.impl("wkv6_bwd", wkv6_bwd);
   m.impl("wkv6_fwd_varlen", wkv6_fwd_varlen);
   m.impl("wkv6_bwd_varlen", wkv6_bwd_varlen);
+  m.impl("linattn_fwd", linattn_fwd);
+  m.impl("linattn_bwd", linattn_bwd);
+  m.impl("linattn_step", linattn_step);
+  m.impl("reorder_states", reorder_states);
+  m.impl("beam_select", beam_select);
 }
 
 TORCH_LIBRARY_IMPL(rwkv_ops_b200, Autograd, m) {
@@ -836,4 +1059,9 @@ TORCH_LIBRARY_IMPL(rwkv_ops_b200, Autograd, m) {
   m.impl("rwkv7_fused_bwd", Gradient<RWKV7_FUSED_BWD, rwkv7_fused_bwd>::call);
   m.impl("wkv6_bwd", Gradient<WKV6_BWD, wkv6_bwd>::call);
   m.impl("wkv6_bwd_varlen", Gradient<WKV6_BWD_VARLEN, wkv6_bwd_varlen>::call);
+  m.impl("linattn_fwd", linattn_fwd_autograd);
+  m.impl("linattn_step", linattn_step_autograd);
+  m.impl("reorder_states", reorder_states_autograd);
+  m.impl("beam_select", beam_select_autograd);
+  m.impl("linattn_bwd", Gradient<LINATTN_BWD, linattn_bwd>::call);
 }

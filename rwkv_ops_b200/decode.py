@@ -14,6 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib, _ops
+from .linear_attention import reorder_states
 
 HEAD_SIZE = 64
 
@@ -59,6 +60,11 @@ class Rwkv7DecodeState:
         except Exception as e:
             self._check_args(r, w, k, v, a, b)
             raise _ops.failed(e)
+
+    def reorder(self, parents: torch.Tensor) -> None:
+        """The states follow a beam search: sequence ``j`` of each search takes the state that sequence ``parents[j]`` of that search had
+        (``parents`` ``[searches, beams]``, at most 32 beams, the beams of a search next to each other in the batch), in place."""
+        reorder_states(self.state, parents)
 
     def final_state(self) -> torch.Tensor:
         """The state as the operator would return it (float32 copy)."""
