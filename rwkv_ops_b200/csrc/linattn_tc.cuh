@@ -48,55 +48,94 @@ __device__ __forceinline__ RawW load_w(const Tokens& t, const float* w, long lon
   return x;
 }
 // by one warp; tokens from n on do not decay.  g (may be NULL): the tokens' g
+// (g is a float32 exponential and only its sums are float64: an error of 2^-23 of L, times e^L, is never more than 2^-24.  With exponentials in float64
+// this took 5000 cycles of its warp, for which the others waited.)
 __device__ __forceinline__ void make_decays(Decays& d, const RawW& x, int n, float* g) {
   const int lane = threadIdx.x & 31;
-  constexpr double LOG2E64 = 1.4426950408889634;
+  float y[4];
   double L[4], s = 0.0;
 #pragma unroll
+  for (int q = 0; q < 4; ++q) y[q] = 4 * lane + q < n ? fmaxf(-expf(x.w[q]), (float)G_FLOOR) : 0.f;
+  if (g) *reinterpret_cast<float4*>(g + 4 * lane) = make_float4(y[0], y[1], y[2], y[3]);
+#pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const double y = 4 * lane + q < n ? g_of(x.w[q]) : 0.0;
-    if (g) g[4 * lane + q] = (float)y;
-    s += y * LOG2E64;      // all in units of log 2 from here on
+    s += (double)y[q];
     L[q] = s;
   }
   double up = s;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
-    const double y = __shfl_up_sync(0xffffffffu, up, m);
-    if (lane >= m) up += y;
+    const double z = __shfl_up_sync(0xffffffffu, up, m);
+    if (lane >= m) up += z;
   }
   const double before = up - s;      // sums of the lanes before
+  constexpr double LOG2E64 = 1.4426950408889634;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) L[q] += before;
-  const double Lc = __shfl_sync(0xffffffffu, L[3], 31);
+  for (int q = 0; q < 4; ++q) L[q] = (L[q] + before) * LOG2E64;      // in units of log 2 from here on
+  // Prefix sums up to the ends of the blocks of 32 tokens; a token's distances to the start and to the end of its own block are all the exponentials it
+  // takes, the others are these times the blocks' own.
+  const double e0 = __shfl_sync(0xffffffffu, L[3], 7), e1 = __shfl_sync(0xffffffffu, L[3], 15), e2 = __shfl_sync(0xffffffffu, L[3], 23),
+               e3 = __shfl_sync(0xffffffffu, L[3], 31);
   const int I = lane >> 3;
-  const double b1 = __shfl_sync(0xffffffffu, L[3], 7), b2 = __shfl_sync(0xffffffffu, L[3], 15), b3 = __shfl_sync(0xffffffffu, L[3], 23);
-  const double mine = I == 0 ? 0.0 : I == 1 ? b1 : I == 2 ? b2 : b3;
+  const double from = I == 0 ? 0.0 : I == 1 ? e0 : I == 2 ? e1 : e2, to = I == 0 ? e0 : I == 1 ? e1 : I == 2 ? e2 : e3;
+  float in[4], low[4], row[4], tail[4];
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const int i = 4 * lane + q;
-    d.start[i] = exp2f((float)L[q]);
-    d.end[i] = exp2f((float)(Lc - L[q]));
-    const float in = (float)(L[q] - mine);
-    d.in[i] = in;
-    d.in_lo[i] = (float)(L[q] - mine - (double)in);
-    d.row[i] = exp2f(in);
-    d.col[0][i] = exp2f((float)fmin(b1 - L[q], 0.0));
-    d.col[1][i] = exp2f((float)fmin(b2 - L[q], 0.0));
-    d.col[2][i] = exp2f((float)fmin(b3 - L[q], 0.0));
+    const double z = L[q] - from;
+    in[q] = (float)z;
+    low[q] = (float)(z - (double)in[q]);
+    row[q] = ex2(in[q]);
+    tail[q] = ex2((float)(to - L[q]));
   }
-  if (lane == 0) d.all = exp2f((float)Lc);
+  const float head = ex2((float)from), rest = ex2((float)(e3 - to));      // of the tokens before, behind this block
+  const float gap1 = ex2((float)(e1 - e0)), gap2 = ex2((float)(e2 - e1));
+  // from the end of this block to the start of block 1, 2, 3 (those behind it)
+  const float c1 = 1.f, c2 = I == 0 ? gap1 : 1.f, c3 = I == 0 ? gap1 * gap2 : I == 1 ? gap2 : 1.f;
+  const auto put = [&](float* p, const float (&v)[4], float f) {
+    *reinterpret_cast<float4*>(p + 4 * lane) = make_float4(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+  };
+  put(d.start, row, head);
+  put(d.end, tail, rest);
+  put(d.row, row, 1.f);
+  put(d.in, in, 1.f);
+  put(d.in_lo, low, 1.f);
+  put(d.col[0], tail, c1);
+  put(d.col[1], tail, c2);
+  put(d.col[2], tail, c3);
+  if (lane == 0) d.all = ex2((float)e3);
 }
 
-// The 32 factors of a row of a diagonal block (those above the diagonal mean nothing): e^{L_i - L_j}.
-__device__ __forceinline__ void diagonal_factors(const Decays& d, int row, int first, float (&f)[32]) {
+// 16 factors of a row of a diagonal block, columns first .. first + 15: e^{L_i - L_j} (those above the diagonal mean nothing).
+__device__ __forceinline__ void diagonal_factors(const Decays& d, int row, int first, float (&f)[16]) {
   const float hi = d.in[row], lo = d.in_lo[row];
 #pragma unroll
-  for (int j = 0; j < 32; j += 4) {
+  for (int j = 0; j < 16; j += 4) {
     const float4 h = *reinterpret_cast<const float4*>(d.in + first + j), l = *reinterpret_cast<const float4*>(d.in_lo + first + j);
     f[j] = ex2((hi - h.x) + (lo - l.x)); f[j + 1] = ex2((hi - h.y) + (lo - l.y));
     f[j + 2] = ex2((hi - h.z) + (lo - l.z)); f[j + 3] = ex2((hi - h.w) + (lo - l.w));
   }
+}
+// and of a block I below the diagonal
+__device__ __forceinline__ void block_factors(const Decays& d, int row, int I, int first, float (&f)[16]) {
+  const float fr = d.row[row];
+#pragma unroll
+  for (int j = 0; j < 16; j += 4) {
+    const float4 g = *reinterpret_cast<const float4*>(d.col[I - 1] + first + j);
+    f[j] = fr * g.x; f[j + 1] = fr * g.y; f[j + 2] = fr * g.z; f[j + 3] = fr * g.w;
+  }
+}
+
+// The kept states are [unit][chunk][4096] in an order of their own: what the 16 lanes that hold 16 rows read or write at once lies together.  Offset of
+// columns 4 c .. 4 c + 3 of row 16 wq + l.
+__device__ __forceinline__ int kept_at(int c, int wq, int l) { return ((c * 4 + wq) * 16 + l) * 4; }
+
+// 16 results of a row to memory as bfloat16: the last rows of a sequence of a packed batch, behind which the next one's lie.  Whole chunks are staged in
+// shared memory and leave by TMA: an SM gets rid of some 16 bytes a cycle, and the threads do not wait for that.
+__device__ __forceinline__ void store_row16(bf16* p, const float (&y)[16]) {
+#pragma unroll
+  for (int j = 0; j < 16; j += 8)
+    *reinterpret_cast<uint4*>(p + j) = make_uint4(pack_bf16(y[j], y[j + 1]), pack_bf16(y[j + 2], y[j + 3]), pack_bf16(y[j + 4], y[j + 5]),
+                                                  pack_bf16(y[j + 6], y[j + 7]));
 }
 
 // Stretches of the units of a call.

@@ -9,6 +9,8 @@ namespace la {
 namespace {
 
 constexpr int NTHR = 256;
+// The two warps that have no block of A on or below the diagonal issue products and copies, and make the next chunk's decays.
+constexpr int ISSUE = 5, DECAYS = 4;
 
 struct FwdSmem {
   unsigned char r[TOK_BYTES], k[TOK_BYTES], v[TOK_BYTES];      // k becomes the hi part of e^{Lc - L_j} k_j
@@ -52,7 +54,7 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
   const uint32_t tm = sm.tmem_base;
   const Stretch x = stretch_of(tok, cut);
   const int seq0 = PACKED ? __ldg(tok.start + x.n) : 0, brow = PACKED ? 0 : x.n;
-  const long long wb = tok.wbase(x.n, x.h);
+  const long long wb = tok.wbase(x.n, x.h), at = tok.base(x.n, x.h) + (long long)row * tok.st + 32 * half;      // of w; of this thread's part of a row
   auto rows_of = [&](int c) { return min(CT, x.len - c * CT); };
   auto load_in = [&](int c) {      // one thread
     const int t0 = seq0 + c * CT;
@@ -62,6 +64,15 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
       tma_load_4d(sm.k + q * TILE_BYTES, &map_k, &sm.bar_in, 0, t0 + 64 * q, x.h, brow);
       if constexpr (!ADD) tma_load_4d(sm.r + q * TILE_BYTES, &map_r, &sm.bar_in, 0, t0 + 64 * q, x.h, brow);
       tma_load_4d(sm.v + q * TILE_BYTES, &map_v, &sm.bar_in, 0, t0 + 64 * q, x.h, brow);
+    }
+  };
+  auto prefetch_in = [&](int c) {
+    const int t0 = seq0 + c * CT;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      tma_prefetch_4d(&map_k, 0, t0 + 64 * q, x.h, brow);
+      if constexpr (!ADD) tma_prefetch_4d(&map_r, 0, t0 + 64 * q, x.h, brow);
+      tma_prefetch_4d(&map_v, 0, t0 + 64 * q, x.h, brow);
     }
   };
   // the state: lanes 0 .. 15 hold row v = 16 wq + lane, columns 32 half .. + 31
@@ -75,21 +86,18 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
 #pragma unroll
     for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(to + sat + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
   };
+  auto keep_state = [&](int c) {
+    float* to = states + ((long long)x.unit * tok.NT + c) * 4096;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(to + kept_at(8 * half + j, wq, lane)) = make_float4(S[4 * j], S[4 * j + 1], S[4 * j + 2], S[4 * j + 3]);
+  };
   bool ok = true;
   float decay = 1.f;
   const int n_chunks = x.hi - x.lo;
   auto chunk = [&](int i) { return REV ? x.hi - 1 - i : x.lo + i; };      // the i-th
   if (n_chunks > 0) {
-    if (warp == 0 && elect_one()) load_in(chunk(0));
-    RawW raw;
-    auto load_raw = [&](int i) {
-      if (i < n_chunks) raw = load_w(tok, w, wb, chunk(i) * CT, rows_of(chunk(i)));
-    };
-    if (warp == 4) {      // the decays are this warp's job: it has no block of A below the diagonal in its half
-      load_raw(0);
-      make_decays(sm.dec[0], raw, rows_of(chunk(0)), nullptr);
-      load_raw(1);
-    }
+    if (warp == ISSUE && elect_one()) load_in(chunk(0));
+    if (warp == DECAYS) make_decays(sm.dec[0], load_w(tok, w, wb, chunk(0) * CT, rows_of(chunk(0))), rows_of(chunk(0)), nullptr);
     if constexpr (!ADD) {
       if (st_lane) {
         const float* from = x.part ? part_states + ((long long)x.unit * cut.parts + x.part) * 4096
@@ -101,17 +109,19 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
             S[j] = f.x; S[j + 1] = f.y; S[j + 2] = f.z; S[j + 3] = f.w;
           }
         }
-        if (states) put_state(states + ((long long)x.unit * tok.NT + x.lo) * 4096);
+        if (states) keep_state(x.lo);
         tile_store_row32(sm.S, srow, 32 * half, S);
       }
-      // A above the diagonal of blocks: never written again
-      for (int e = tid; e < CT * 8; e += NTHR) *reinterpret_cast<uint4*>(sm.A[1] + 16 * e) = make_uint4(0, 0, 0, 0);
+      // A above the diagonal of blocks: never written to again
+      for (int e = tid; e < 2 * CT * 8; e += NTHR) *reinterpret_cast<uint4*>(sm.A[0] + 16 * e) = make_uint4(0, 0, 0, 0);
     }
     fence_async_smem();
     __syncthreads();
     for (int i = 0; i < n_chunks; ++i) {
       const int c = chunk(i);
       const uint32_t ph = i & 1;
+      RawW raw;      // w of the next chunk
+      if (warp == DECAYS && i + 1 < n_chunks) raw = load_w(tok, w, wb, chunk(i + 1) * CT, rows_of(chunk(i + 1)));
       const Decays& d = sm.dec[ph];
       const int n = rows_of(c);
       ok = mbar_wait(&sm.bar_in, ph, status, 501) && ok;
@@ -122,14 +132,15 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
         __syncthreads();
       }
       if constexpr (!ADD) {
-        if (warp == 0 && elect_one()) {
-          bulk_wait_read();      // o of the chunk before has left its place in A
+        if (warp == ISSUE && elect_one()) {
           tc_fence_after();
           umma_tile<128, 128, 0, 0>(tmem_addr(tm, 0, TM_S), smem_u32(sm.r), smem_u32(sm.k), false);
+          bulk_wait_read();            // o of the chunk before has left its place in A, which is written to after these products
+          umma_commit(&sm.bar_1);      // (the products with the state run on under what the threads do with these)
           umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_O1), smem_u32(sm.r), smem_u32(sm.S), false);
-          umma_commit(&sm.bar_1);
         }
       }
+      if (i + 1 < n_chunks && warp == ISSUE && elect_one()) prefetch_in(chunk(i + 1));
       // scaled keys, 32 columns of a token; the hi part waits until the products have read the keys as they are
       uint4 hi[4];
       {
@@ -167,42 +178,36 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const int J = 2 * half + b;
-          float p[32];
           if (J <= wq) {
-            uint32_t s[32];
-            tmem_ld32(tmem_addr(tm, 32 * wq, TM_S + 32 * J), s);
-            if (J < wq) {
-              const float f = d.row[row];
-              const float* col = d.col[wq - 1] + 32 * J;
-              tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 32; j += 4) {
-                const float4 g = *reinterpret_cast<const float4*>(col + j);
-                p[j] = __uint_as_float(s[j]) * (f * g.x); p[j + 1] = __uint_as_float(s[j + 1]) * (f * g.y);
-                p[j + 2] = __uint_as_float(s[j + 2]) * (f * g.z); p[j + 3] = __uint_as_float(s[j + 3]) * (f * g.w);
+            for (int h = 0; h < 2; ++h) {      // 16 columns at a time: registers (a spilled one goes to L2, there is no L1 left)
+              uint32_t s[16];
+              float p[16];
+              tmem_ld16(tmem_addr(tm, 32 * wq, TM_S + 32 * J + 16 * h), s);
+              if (J < wq) {
+                block_factors(d, row, wq, 32 * J + 16 * h, p);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) p[j] *= __uint_as_float(s[j]);
+              } else {
+                diagonal_factors(d, row, 32 * J + 16 * h, p);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) p[j] = 16 * h + j <= lane ? __uint_as_float(s[j]) * p[j] : 0.f;
               }
-            } else {
-              diagonal_factors(d, row, 32 * J, p);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 32; ++j) p[j] = j <= lane ? __uint_as_float(s[j]) * p[j] : 0.f;
+              tile_store_row<16>(At, row & 63, 32 * b + 16 * h, p);
             }
-            tile_store_row32(At, row & 63, 32 * b, p);
           } else if (J == 1) {      // (wq == 0: the staged o was here)
 #pragma unroll
-            for (int j = 0; j < 32; ++j) p[j] = 0.f;
-            tile_store_row32(At, row & 63, 32 * b, p);
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<uint4*>(At + tile_chunk_off(row & 63, 4 * b + q)) = make_uint4(0, 0, 0, 0);
           }
         }
       }
-      if (warp == 4 && i + 1 < n_chunks) {
-        make_decays(sm.dec[ph ^ 1], raw, rows_of(chunk(i + 1)), nullptr);
-        load_raw(i + 2);
-      }
+      if (warp == DECAYS && i + 1 < n_chunks) make_decays(sm.dec[ph ^ 1], raw, rows_of(chunk(i + 1)), nullptr);
       fence_async_smem();
       tc_fence_before();
       __syncthreads();
-      if (warp == 0 && elect_one()) {
+      if (warp == ISSUE && elect_one()) {
         tc_fence_after();
         if constexpr (!ADD) {
           umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_O2), smem_u32(sm.A[0]), smem_u32(sm.v), false);
@@ -214,7 +219,7 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
       }
       ok = mbar_wait(&sm.bar_2, ph, status, 503) && ok;
       tc_fence_after();
-      if (i + 1 < n_chunks && warp == 0 && elect_one()) load_in(chunk(i + 1));
+      if (i + 1 < n_chunks && warp == ISSUE && elect_one()) load_in(chunk(i + 1));
       const float all = d.all;
       {
         uint32_t u[32];
@@ -228,33 +233,31 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
       } else {
         if (st_lane) {
           tile_store_row32(sm.S, srow, 32 * half, S);
-          if (states && c + 1 < x.hi) put_state(states + ((long long)x.unit * tok.NT + c + 1) * 4096);
+          if (states && c + 1 < x.hi) keep_state(c + 1);
         }
-        uint32_t a[32], b[32];
-        tmem_ld32(tmem_addr(tm, 32 * wq, TM_O1 + 32 * half), a);
-        tmem_ld32(tmem_addr(tm, 32 * wq, TM_O2 + 32 * half), b);
-        tmem_ld_wait();
         const float f = d.start[row];
-        float y[32];
+        bf16* to = o + at + (long long)(c * CT) * tok.st;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) y[j] = fmaf(f, __uint_as_float(a[j]), __uint_as_float(b[j]));
-        if (!o) {                    // (the states alone)
-        } else if (PACKED && n < CT) {      // the rows behind belong to the next sequence
-          if (row < n) {
-            bf16* to = o + tok.base(x.n, x.h) + (long long)(c * CT + row) * tok.st + 32 * half;
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a[16], b[16];
+          tmem_ld16(tmem_addr(tm, 32 * wq, TM_O1 + 32 * half + 16 * h), a);
+          tmem_ld16(tmem_addr(tm, 32 * wq, TM_O2 + 32 * half + 16 * h), b);
+          tmem_ld_wait();
+          float y[16];
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              *reinterpret_cast<uint4*>(to + j) = make_uint4(pack_bf16(y[j], y[j + 1]), pack_bf16(y[j + 2], y[j + 3]),
-                                                             pack_bf16(y[j + 4], y[j + 5]), pack_bf16(y[j + 6], y[j + 7]));
+          for (int j = 0; j < 16; ++j) y[j] = fmaf(f, __uint_as_float(a[j]), __uint_as_float(b[j]));
+          if (!o) continue;      // (the states alone)
+          if (PACKED && n < CT) {
+            if (row < n) store_row16(to + 16 * h, y);
+          } else {
+            tile_store_row<16>(sm.A[0] + (row >> 6) * TILE_BYTES, row & 63, 32 * half + 16 * h, y);
           }
-        } else {
-          tile_store_row32(sm.A[0] + (row >> 6) * TILE_BYTES, row & 63, 32 * half, y);
         }
       }
       fence_async_smem();
       tc_fence_before();
       if (!__syncthreads_and(ok)) break;
-      if (!ADD && o && !(PACKED && n < CT) && warp == 0 && elect_one()) {
+      if (!ADD && o && !(PACKED && n < CT) && warp == ISSUE && elect_one()) {
 #pragma unroll
         for (int q = 0; q < 2; ++q)      // (rows past the end of the batch are clipped)
           if (64 * q < n) tma_store_4d(&map_o, sm.A[0] + q * TILE_BYTES, 0, seq0 + c * CT + 64 * q, x.h, brow);
@@ -273,7 +276,7 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
   } else {
     if (st_lane && ht && (x.NT == 0 ? x.part == 0 : x.lo < x.hi && x.hi == x.NT)) put_state(ht + (long long)x.unit * 4096);
   }
-  if (warp == 0 && elect_one()) bulk_wait_all();
+  if (warp == ISSUE && elect_one()) bulk_wait_all();
   tc_fence_before();
   __syncthreads();
   if (warp == 0) tmem_dealloc(tm, TM_COLS);
@@ -326,12 +329,11 @@ int fwd(const Args& a, cudaStream_t st) {
   if (int e = allow_smem<la_tc_fwd_kernel<PACKED, true>>(f, smem)) return e;
   const int B = t.start ? 1 : t.n_seq, T = t.start ? (int)a.w_rows : t.T, head_first = t.st == 64 && t.H > 1;
   CUtensorMap mr, mk, mv, mo;
-  const void* r = a.r ? a.r : a.k;      // (the states alone: r is not loaded, o not stored)
-  void* o = a.o ? a.o : const_cast<void*>(a.k);
+  const void* r = a.r ? a.r : a.k;      // (the states alone: whatever r k^T is, it goes nowhere)
   if (int e = make_token_tensor_map(&mr, r, B, T, t.H, head_first)) return e;
   if (int e = make_token_tensor_map(&mk, a.k, B, T, t.H, head_first)) return e;
   if (int e = make_token_tensor_map(&mv, a.v, B, T, t.H, head_first)) return e;
-  if (int e = make_token_tensor_map(&mo, o, B, T, t.H, head_first)) return e;
+  if (int e = make_token_tensor_map(&mo, a.o ? a.o : a.k, B, T, t.H, head_first)) return e;
   const Cut cut = cut_units(t.n_seq, t.T, t.H, false);
   float* part_states = static_cast<float*>(a.scratch);
   float* part_decay = part_states + (size_t)cut.n_units * cut.parts * 4096;
