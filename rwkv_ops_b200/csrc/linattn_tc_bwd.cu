@@ -27,9 +27,9 @@ struct BwdSmem {
   uint32_t tmem_base;
 };
 // The warps whose block of pairs lies above the diagonal (4, 8, 9, 12, 13, 14) do the other jobs: ISSUE the products (a thread that issues is held up by those
-// under way, some 50 cycles each), STORE the copies of the gradients, DECAYS the next chunk's decays, DW the dw of the chunk before, and STORE, ISSUE_W and
-// 13 the scaled r.
-constexpr int ISSUE = 14, STORE = 4, DECAYS = 8, DW = 12, ISSUE_W = 9, SCALE = 13, SCALE_WARPS = 3;
+// under way, some 50 cycles each), STORE the copies of the gradients, DECAYS the next chunk's decays, DW the dw of the chunk before and (LOAD) the loads, and
+// STORE, ISSUE_W and 13 the scaled r.
+constexpr int ISSUE = 14, STORE = 4, DECAYS = 8, LOAD = 12, DW = 12, ISSUE_W = 9, SCALE = 13, SCALE_WARPS = 3;
 constexpr uint32_t TM_S = 0, TM_P = 128, TM_YR = 0, TM_YK = 64, TM_YV = 128, TM_XR = 256, TM_XK = 320, TM_XV = 384, TM_W = 448, TM_COLS = 512;
 
 // the sum over a warp's lanes of x[c], in lanes c and c + 16
@@ -227,7 +227,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
     if (dw_parts) sm.dw_sum[lane] += (double)part;
   };
   if (x.lo < x.hi) {
-    if (warp == ISSUE && elect_one()) load_in(x.hi - 1);
+    if (warp == LOAD && elect_one()) load_in(x.hi - 1);
     if (warp == DECAYS) {
       make_decays(sm.dec[0], load_w(tok, w, wb, (x.hi - 1) * CT, rows_of(x.hi - 1)), rows_of(x.hi - 1), sm.g[0]);
       if (lane == 0) sm.decay[0] = sm.dec[0].all;
@@ -345,25 +345,6 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
         }
         if (warp == DW && i) write_dw(c + 1, i - 1);
         ok = mbar_wait(&sm.bar_free, ph, status, 518) && ok;      // (the gradients of the chunk before were staged in what follows)
-        if (warp == STORE || warp == ISSUE_W || warp == SCALE) {      // 16 bytes of r at a time
-          for (int e = lane + 32 * (warp == STORE ? 0 : warp == ISSUE_W ? 1 : 2); e < CT * 8; e += 32 * SCALE_WARPS) {
-            const int t = e >> 3;
-            const float f = d.start[t];
-            const uint32_t off = (t >> 6) * TILE_BYTES + tile_chunk_off(t & 63, e & 7);
-            const uint4 u = *reinterpret_cast<const uint4*>(sm.r + off);
-            const uint32_t in[4] = {u.x, u.y, u.z, u.w};
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const float a = bf16_lo(in[q]) * f, b = bf16_hi(in[q]) * f;
-              hi[q] = pack_bf16(a, b);
-              lo[q] = pack_bf16(a - bf16_lo(hi[q]), b - bf16_hi(hi[q]));
-            }
-            *reinterpret_cast<uint4*>(sm.rhi + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(sm.rlo + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          }
-          arrive(sm.bar_r);
-        }
         const uint4 z = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -374,14 +355,35 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       }
       tc_fence_before();
       arrive(sm.bar_ae);
-      if (warp == ISSUE_W) {
-        ok = mbar_wait(&sm.bar_r, ph, status, 515) && ok;
-        tc_fence_after();
-        if (elect_one()) {
-          umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.rhi), false);
-          umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.rlo), true);
-          umma_commit(&sm.bar_2);
+      if (warp == STORE || warp == ISSUE_W || warp == SCALE) {      // the scaled r, 16 bytes of 16 tokens at a time
+        const int first = warp == STORE ? 0 : warp == ISSUE_W ? 48 : 96, n_row = warp == SCALE ? 32 : 48;
+#pragma unroll 2
+        for (int e = lane; e < n_row * 8; e += 64) {
+          uint4 u[2];
+          float f[2];
+          uint32_t off[2];
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int t = first + ((e + 32 * q) >> 3);
+            off[q] = (t >> 6) * TILE_BYTES + tile_chunk_off(t & 63, e & 7);
+            u[q] = *reinterpret_cast<const uint4*>(sm.r + off[q]);
+            f[q] = d.start[t];
+          }
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const uint32_t in[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const float a = bf16_lo(in[g]) * f[q], b = bf16_hi(in[g]) * f[q];
+              hi[g] = pack_bf16(a, b);
+              lo[g] = pack_bf16(a - bf16_lo(hi[g]), b - bf16_hi(hi[g]));
+            }
+            *reinterpret_cast<uint4*>(sm.rhi + off[q]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(sm.rlo + off[q]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          }
         }
+        arrive(sm.bar_r);
       }
       if (c > x.lo) get_kept(c - 1);
       // the states' parts of dr and dk, and of dw
@@ -401,6 +403,15 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       state_part(TM_XK, d.end[row], sm.k, sm.t2[ph][qt]);
       if (c > x.lo && st_lane) store_split16(sm.S[0], sm.S[1], srow, 16 * qt, S0);      // (the products with this chunk's are done)
       arrive(sm.bar_read);
+      if (warp == ISSUE_W) {
+        ok = mbar_wait(&sm.bar_r, ph, status, 515) && ok;
+        tc_fence_after();
+        if (elect_one()) {
+          umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.rhi), false);
+          umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.rlo), true);
+          umma_commit(&sm.bar_2);
+        }
+      }
       if (warp == ISSUE) {
         ok = mbar_wait(&sm.bar_ae, ph, status, 516) && ok;
         tc_fence_after();
@@ -414,7 +425,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       }
       ok = mbar_wait(&sm.bar_2, ph, status, 513) && ok;
       tc_fence_after();
-      if (c > x.lo && warp == ISSUE) {
+      if (c > x.lo && warp == LOAD) {
         ok = mbar_wait(&sm.bar_read, ph, status, 517) && ok;
         if (elect_one()) load_in(c - 1);
       }
