@@ -7,9 +7,8 @@
 // states.  A and E are rounded once to bfloat16, as is the state that meets r in the forward: those results are rounded to bfloat16 anyway.
 //
 // Work is cut into items, a stretch of consecutive chunks of one (sequence, head).  With as many units as the device holds CTAs, an item is a unit.  With
-// fewer, a unit is several stretches: a first kernel walks every stretch from a zero state, keys and values only, a small one chains the stretches' states
-// (elementwise), and then all stretches are walked at once from the state each starts with.  That reads half the tokens twice and pays as soon as
-// the chain of chunks is more than a few.
+// fewer, a unit is several parts: a first kernel finds what each adds to the state, keys and values only, and then all parts are walked at once from the state
+// each starts with.  That reads half of the tokens twice and pays as soon as the chain of chunks is more than a few.
 #pragma once
 
 #include "linattn.cuh"
@@ -138,20 +137,80 @@ __device__ __forceinline__ void store_row16(bf16* p, const float (&y)[16]) {
                                                   pack_bf16(y[j + 6], y[j + 7]));
 }
 
-// Stretches of the units of a call.
+// Stretches of the units of a call: parts of `per` chunks.  What a part starts from is put together from what the parts before it (backward: behind it) add to
+// the state; that is found by a pass of its own over those, each in `sub` pieces of `per_sub` chunks, as there are more SMs than parts.
 struct Cut {
-  int n_units, parts, per;      // parts of `per` chunks
+  int n_units, parts, per, sub, per_sub;
+  __host__ __device__ int adds() const { return (parts - 1) * sub; }      // of a unit
+  bool chained() const { return adds() > 12; }      // put together by a kernel of its own; otherwise by each part, at its start
 };
 struct Stretch { int unit, part, n, h, len, NT, lo, hi; };
-__device__ __forceinline__ Stretch stretch_of(const Tokens& t, const Cut& cut) {
+__device__ __forceinline__ Stretch unit_of(const Tokens& t, const Cut& cut) {
   Stretch x;
   x.unit = blockIdx.x % cut.n_units; x.part = blockIdx.x / cut.n_units;
   x.n = x.unit / t.H; x.h = x.unit % t.H;
   x.len = t.length(x.n);
   x.NT = (x.len + CT - 1) / CT;
+  return x;
+}
+__device__ __forceinline__ Stretch stretch_of(const Tokens& t, const Cut& cut) {
+  Stretch x = unit_of(t, cut);
   x.lo = min(x.part * cut.per, x.NT);
   x.hi = min(x.lo + cut.per, x.NT);
   return x;
+}
+// a piece of the pass that adds: `part` counts the pieces of a unit, in the order of the chunks
+__device__ __forceinline__ Stretch piece_of(const Tokens& t, const Cut& cut, bool reverse) {
+  Stretch x = unit_of(t, cut);
+  const int p = x.part / cut.sub + reverse, s = x.part % cut.sub;
+  x.lo = min(p * cut.per + s * cut.per_sub, x.NT);
+  x.hi = min(min(x.lo + cut.per_sub, (p + 1) * cut.per), x.NT);
+  return x;
+}
+
+// Memory of a call that has parts: what the pieces add [unit][adds] and their decays, and (chained) what the parts start from [unit][parts].  All states in the order of
+// kept_at().
+struct Pieces { float *add, *start, *decay; };
+inline size_t pieces_bytes(const Cut& c) {
+  if (c.parts == 1) return 0;
+  return ((size_t)c.n_units * (c.adds() + (c.chained() ? c.parts : 0)) * 4096 + (size_t)c.n_units * c.adds()) * 4;
+}
+inline Pieces pieces_at(void* p, const Cut& c) {
+  Pieces x;
+  x.add = static_cast<float*>(p);
+  x.start = x.add + (size_t)c.n_units * c.adds() * 4096;
+  x.decay = x.start + (size_t)c.n_units * (c.chained() ? c.parts : 0) * 4096;
+  return x;
+}
+// The state that a part of a unit starts from (reverse: its gradient behind the part): N / 4 pieces of four columns of a row from c0 on.
+template <int N>
+__device__ __forceinline__ void start_of(float (&S)[N], const Stretch& x, const Cut& cut, bool reverse, bool chained, const float* add, const float* start,
+                                         const float* decay, const float* first, int c0, int wq, int lane) {
+  const bool have = lane < 16;      // (the lanes that hold a row)
+  if (x.part == (reverse ? cut.parts - 1 : 0) || !chained) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      const float4 f = have && first ? __ldcg(reinterpret_cast<const float4*>(first + (16 * wq + lane) * 64 + 4 * c0 + j)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      S[j] = f.x; S[j + 1] = f.y; S[j + 2] = f.z; S[j + 3] = f.w;
+    }
+    const int n = reverse ? (cut.parts - 1 - x.part) * cut.sub : x.part * cut.sub;
+    for (int i = 0; i < n; ++i) {
+      const int a = x.unit * cut.adds() + (reverse ? cut.adds() - 1 - i : i);
+      const float d = __ldcg(decay + a);
+#pragma unroll
+      for (int j = 0; j < N; j += 4) {
+        const float4 f = have ? __ldcg(reinterpret_cast<const float4*>(add + (long long)a * 4096 + kept_at(c0 + j / 4, wq, lane))) : make_float4(0.f, 0.f, 0.f, 0.f);
+        S[j] = fmaf(d, S[j], f.x); S[j + 1] = fmaf(d, S[j + 1], f.y); S[j + 2] = fmaf(d, S[j + 2], f.z); S[j + 3] = fmaf(d, S[j + 3], f.w);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      const float4 f = have ? __ldcg(reinterpret_cast<const float4*>(start + (long long)(x.unit * cut.parts + x.part) * 4096 + kept_at(c0 + j / 4, wq, lane)))
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
+      S[j] = f.x; S[j + 1] = f.y; S[j + 2] = f.z; S[j + 3] = f.w;
+    }
+  }
 }
 
 // rows n .. 127 of a chunk's token tile (they belong to the next sequence of a packed batch) as zeros
@@ -160,12 +219,8 @@ __device__ __forceinline__ void zero_rows(unsigned char* tile, int n) {
 }
 
 Cut cut_units(int n_seq, int max_len, int H, bool backward);
-// the states (or their gradients) that the stretches start from, from what each adds; defined beside the forward
-int launch_chain(float* part_states, const float* part_decay, const float* first, int n_first, const Tokens& t, const Cut& cut, bool reverse,
-                 cudaStream_t st);
-
-// what every stretch adds to the gradient of the state before it (values d_o, keys r), walking backwards
-int launch_tc_add(const Args& a, const Cut& cut, const CUtensorMap& map_do, const CUtensorMap& map_r, float* part_states, float* part_decay, int* status,
+// what the pieces add, and (chained) what the parts start from; values v and keys k, or backwards d_o and r
+int launch_pieces(const Args& a, const Cut& cut, const CUtensorMap& map_val, const CUtensorMap& map_key, const Pieces& p, bool reverse, int* status,
                   cudaStream_t st);
 
 }  // namespace la

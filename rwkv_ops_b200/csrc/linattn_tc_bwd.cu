@@ -73,7 +73,8 @@ template <bool PACKED>
 __global__ void __launch_bounds__(NTHR, 1)
 la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, const float* __restrict__ states, bf16* __restrict__ dr,
                  bf16* __restrict__ dk, bf16* __restrict__ dv, float* __restrict__ dw, int dw_parts, float* __restrict__ dh0,
-                 const float* __restrict__ part_states, const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_k,
+                 const float* __restrict__ add, const float* __restrict__ start, const float* __restrict__ decay, int chained,
+                 const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_k,
                  const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_do,
                  const __grid_constant__ CUtensorMap map_dr, const __grid_constant__ CUtensorMap map_dk, const __grid_constant__ CUtensorMap map_dv,
                  Tokens tok, Cut cut, int* status) {
@@ -145,13 +146,6 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
   const int srow = 16 * wq + (lane & 15);
   const long long sat = (long long)srow * 64 + 16 * qt;
   float dS[16], S0[16];
-  auto get_state = [&](float (&s)[16], const float* from) {
-#pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-      const float4 f = st_lane && from ? __ldcg(reinterpret_cast<const float4*>(from + sat + j)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      s[j] = f.x; s[j + 1] = f.y; s[j + 2] = f.z; s[j + 3] = f.w;
-    }
-  };
   auto get_kept = [&](int c) {
     const float* from = states + ((long long)x.unit * tok.NT + c) * 4096;
 #pragma unroll
@@ -172,7 +166,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
     for (int m = 8; m >= 1; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
     if (lane == 0) sm.t3[ph][warp] = s;
   };
-  get_state(dS, x.part + 1 < cut.parts ? part_states + ((long long)x.unit * cut.parts + x.part) * 4096 : d_ht ? d_ht + (long long)x.unit * 4096 : nullptr);
+  start_of(dS, x, cut, true, chained, add, start, decay, d_ht ? d_ht + (long long)x.unit * 4096 : nullptr, 4 * qt, wq, lane);
   bool ok = true;
   if (warp == DW) sm.dw_sum[lane] = 0.0;
   // dw of chunk c, the i-th of the stretch, by one warp: four tokens to a lane
@@ -495,20 +489,19 @@ int bwd(const Args& a, cudaStream_t st) {
   for (int i = 0; i < 7; ++i)
     if (int e = make_token_tensor_map(&m[i], in[i], B, T, t.H, head_first)) return e;
   const Cut cut = cut_units(t.n_seq, t.T, t.H, true);
-  float* part_states = static_cast<float*>(a.scratch);
-  float* part_decay = part_states + (size_t)cut.n_units * cut.parts * 4096;
-  const size_t chain = cut.parts > 1 ? (size_t)cut.n_units * cut.parts * (4096 + 1) * 4 : 0;
+  const Pieces p = pieces_at(a.scratch, cut);
+  const size_t chain = pieces_bytes(cut);
   float* dw_rows = reinterpret_cast<float*>(static_cast<unsigned char*>(a.scratch) + (chain + 255) / 256 * 256);      // [n_seq][parts][H]
   const size_t n_rows = (size_t)t.n_seq * cut.parts;
   double* dw_part = reinterpret_cast<double*>(reinterpret_cast<unsigned char*>(dw_rows) + (n_rows * t.H * 4 + 255) / 256 * 256);
   if (cut.parts > 1) {
-    if (int e = launch_tc_add(a, cut, m[3], m[0], part_states, part_decay, f.status, st)) return e;
-    if (int e = launch_chain(part_states, part_decay, a.d_ht, t.n_seq, t, cut, true, st)) return e;
+    if (int e = launch_pieces(a, cut, m[3], m[0], p, true, f.status, st)) return e;
   }
   {
     ProfScope prof("linattn_tc_bwd_kernel", st);
     if (int e = launch(la_tc_bwd_kernel<PACKED>, cut.n_units * cut.parts, NTHR, smem, st, 1, a.w, a.d_ht, (const float*)a.states, (bf16*)a.dr, (bf16*)a.dk,
-                       (bf16*)a.dv, a.w_per_head ? dw_rows : a.dw, a.w_per_head, a.dh0, (const float*)part_states, m[0], m[1], m[2], m[3], m[4], m[5],
+                       (bf16*)a.dv, a.w_per_head ? dw_rows : a.dw, a.w_per_head, a.dh0, (const float*)p.add,
+                       (const float*)p.start, (const float*)p.decay, (int)cut.chained(), m[0], m[1], m[2], m[3], m[4], m[5],
                        m[6], t, cut, f.status)) return e;
   }
   return a.w_per_head ? launch_sum_dw(dw_rows, (long long)n_rows, t.H, dw_part, a.dw, st) : RWKVB200_OK;

@@ -21,23 +21,31 @@ struct FwdSmem {
   uint64_t bar_in, bar_1, bar_2;
   uint32_t tmem_base;
 };
-constexpr uint32_t TM_S = 0, TM_O2 = 0, TM_U = 64, TM_O1 = 128, TM_COLS = 256;
+struct AddSmem {      // keys and values alone: three CTAs to an SM
+  unsigned char k[TOK_BYTES], v[TOK_BYTES], klo[TOK_BYTES];
+  Decays dec[2];
+  uint64_t bar_in, bar_1, bar_2;
+  uint32_t tmem_base;
+};
+constexpr uint32_t TM_S = 0, TM_O2 = 0, TM_O1 = 128;
 
 // One item: the chunks of a stretch in order, the state in registers (a row to the lower half lanes of a warp, 32 columns).  Per chunk two batches of
 // products with the threads' work between them:
 //   r k^T, r S^T            meanwhile the keys are scaled and split
 //   A v, v^T (scaled keys)  after A = (r k^T) * decays has been rounded and stored; then o and the next state
-// ADD: keys and values alone, from a zero state; what the stretch adds and its decay go to part_states / part_decay.  REV: the same for the
+// ADD: keys and values alone, from a zero state; what the piece adds and its decay go to `add` and `decay`.  REV: the same for the
 // gradient of the state, from the last chunk to the first, with r for keys and d_o for values.
 // Two CTAs share an SM (113 KB each, 256 TMEM columns each), so that one's products and loads run under the other's arithmetic.
 template <bool PACKED, bool ADD, bool REV = false>
-__global__ void __launch_bounds__(NTHR, 2)
+__global__ void __launch_bounds__(NTHR, ADD ? 3 : 2)
 la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int n_state, bf16* __restrict__ o, float* __restrict__ ht,
-                 float* __restrict__ states, float* __restrict__ part_states, float* __restrict__ part_decay,
+                 float* __restrict__ states, float* __restrict__ add, const float* __restrict__ start, float* __restrict__ decay, int chained,
                  const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                  const __grid_constant__ CUtensorMap map_o, Tokens tok, Cut cut, int* status) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  FwdSmem& sm = *reinterpret_cast<FwdSmem*>(smem_raw);
+  typedef std::conditional_t<ADD, AddSmem, FwdSmem> Smem;
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
+  constexpr uint32_t TM_U = ADD ? 0 : 64, TM_COLS = ADD ? 64 : 256;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wq = warp & 3, half = warp >> 2, row = 32 * wq + lane;      // the token whose row this thread reads, and which half of the columns
   if (tid == 0) {
@@ -52,7 +60,7 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
   earlier_kernels_done();
   later_kernels_may_start();
   const uint32_t tm = sm.tmem_base;
-  const Stretch x = stretch_of(tok, cut);
+  const Stretch x = ADD ? piece_of(tok, cut, REV) : stretch_of(tok, cut);
   const int seq0 = PACKED ? __ldg(tok.start + x.n) : 0, brow = PACKED ? 0 : x.n;
   const long long wb = tok.wbase(x.n, x.h), at = tok.base(x.n, x.h) + (long long)row * tok.st + 32 * half;      // of w; of this thread's part of a row
   auto rows_of = [&](int c) { return min(CT, x.len - c * CT); };
@@ -86,29 +94,21 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
 #pragma unroll
     for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4*>(to + sat + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
   };
-  auto keep_state = [&](int c) {
-    float* to = states + ((long long)x.unit * tok.NT + c) * 4096;
+  auto put_kept = [&](float* to) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(to + kept_at(8 * half + j, wq, lane)) = make_float4(S[4 * j], S[4 * j + 1], S[4 * j + 2], S[4 * j + 3]);
   };
+  auto keep_state = [&](int c) { put_kept(states + ((long long)x.unit * tok.NT + c) * 4096); };
   bool ok = true;
-  float decay = 1.f;
+  float product = 1.f;
   const int n_chunks = x.hi - x.lo;
   auto chunk = [&](int i) { return REV ? x.hi - 1 - i : x.lo + i; };      // the i-th
   if (n_chunks > 0) {
     if (warp == ISSUE && elect_one()) load_in(chunk(0));
     if (warp == DECAYS) make_decays(sm.dec[0], load_w(tok, w, wb, chunk(0) * CT, rows_of(chunk(0))), rows_of(chunk(0)), nullptr);
     if constexpr (!ADD) {
+      start_of(S, x, cut, false, chained, add, start, decay, h0 ? h0 + ((long long)(n_state == 1 ? 0 : x.n) * tok.H + x.h) * 4096 : nullptr, 8 * half, wq, lane);
       if (st_lane) {
-        const float* from = x.part ? part_states + ((long long)x.unit * cut.parts + x.part) * 4096
-                            : h0   ? h0 + ((long long)(n_state == 1 ? 0 : x.n) * tok.H + x.h) * 4096 : nullptr;
-        if (from) {
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 f = __ldcg(reinterpret_cast<const float4*>(from + sat + j));
-            S[j] = f.x; S[j + 1] = f.y; S[j + 2] = f.z; S[j + 3] = f.w;
-          }
-        }
         if (states) keep_state(x.lo);
         tile_store_row32(sm.S, srow, 32 * half, S);
       }
@@ -229,7 +229,7 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
         for (int j = 0; j < 32; ++j) S[j] = fmaf(all, S[j], __uint_as_float(u[j]));
       }
       if constexpr (ADD) {
-        decay *= all;
+        product *= all;
       } else {
         if (st_lane) {
           tile_store_row32(sm.S, srow, 32 * half, S);
@@ -257,11 +257,13 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
       fence_async_smem();
       tc_fence_before();
       if (!__syncthreads_and(ok)) break;
-      if (!ADD && o && !(PACKED && n < CT) && warp == ISSUE && elect_one()) {
+      if constexpr (!ADD) {
+        if (o && !(PACKED && n < CT) && warp == ISSUE && elect_one()) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)      // (rows past the end of the batch are clipped)
-          if (64 * q < n) tma_store_4d(&map_o, sm.A[0] + q * TILE_BYTES, 0, seq0 + c * CT + 64 * q, x.h, brow);
-        bulk_commit();
+          for (int q = 0; q < 2; ++q)      // (rows past the end of the batch are clipped)
+            if (64 * q < n) tma_store_4d(&map_o, sm.A[0] + q * TILE_BYTES, 0, seq0 + c * CT + 64 * q, x.h, brow);
+          bulk_commit();
+        }
       }
     }
   } else if (!ADD && st_lane) {      // no chunk: a sequence without tokens hands its state on
@@ -271,8 +273,8 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
     }
   }
   if constexpr (ADD) {
-    if (st_lane) put_state(part_states + ((long long)x.unit * cut.parts + x.part) * 4096);
-    if (tid == 0) part_decay[(long long)x.unit * cut.parts + x.part] = decay;
+    if (st_lane) put_kept(add + ((long long)x.unit * cut.adds() + x.part) * 4096);
+    if (tid == 0) decay[x.unit * cut.adds() + x.part] = product;
   } else {
     if (st_lane && ht && (x.NT == 0 ? x.part == 0 : x.lo < x.hi && x.hi == x.NT)) put_state(ht + (long long)x.unit * 4096);
   }
@@ -282,35 +284,42 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
   if (warp == 0) tmem_dealloc(tm, TM_COLS);
 }
 
-// part_states[unit][p] becomes the state that stretch p starts from (reverse: the gradient of the state that it ends with), from what each stretch adds.
-__global__ void __launch_bounds__(256) la_chain_kernel(float* __restrict__ part, const float* __restrict__ decay, const float* __restrict__ first,
-                                                       int n_first, int H, int n_units, int parts, int reverse) {
+// What the parts of a unit start from (reverse: the gradient behind them), from what the pieces add; four elements of a state to a thread.
+__global__ void __launch_bounds__(256) la_chain_kernel(const float* __restrict__ add, const float* __restrict__ decay, float* __restrict__ start,
+                                                       const float* __restrict__ first, int n_first, int H, Cut cut, int reverse) {
   earlier_kernels_done();
   later_kernels_may_start();
-  const int i = blockIdx.x * 256 + threadIdx.x, unit = i >> 10, e = 4 * (i & 1023);
-  if (unit >= n_units) return;
+  const int i = blockIdx.x * 256 + threadIdx.x, unit = i >> 10, e = i & 1023;
   float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (first) S = *reinterpret_cast<const float4*>(first + (n_first == 1 ? (long long)(unit % H) : (long long)unit) * 4096 + e);
-  float* p0 = part + (long long)unit * parts * 4096 + e;
+  if (first) {
+    const int c = e >> 6, v = e & 63;      // columns 4 c .. of row v (kept_at)
+    S = *reinterpret_cast<const float4*>(first + (n_first == 1 ? (long long)(unit % H) : (long long)unit) * 4096 + v * 64 + 4 * c);
+  }
+  const int n = cut.adds();
+  const float* a0 = add + (long long)unit * n * 4096 + 4 * e;
+  float* s0 = start + (long long)unit * cut.parts * 4096 + 4 * e;
   constexpr int AHEAD = 8;
-  for (int q0 = 0; q0 < parts; q0 += AHEAD) {
-    float4 add[AHEAD];
-    float f[AHEAD];
+  for (int q0 = 0; q0 < n; q0 += AHEAD) {
+    float4 f[AHEAD];
+    float d[AHEAD];
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
-      if (q0 + q < parts) {
-        const int p = reverse ? parts - 1 - q0 - q : q0 + q;
-        add[q] = *reinterpret_cast<const float4*>(p0 + (long long)p * 4096);
-        f[q] = decay[(long long)unit * parts + p];
+      if (q0 + q < n) {
+        const int a = reverse ? n - 1 - q0 - q : q0 + q;
+        f[q] = *reinterpret_cast<const float4*>(a0 + (long long)a * 4096);
+        d[q] = decay[unit * n + a];
       }
     }
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
-      if (q0 + q < parts) {
-        const int p = reverse ? parts - 1 - q0 - q : q0 + q;
-        *reinterpret_cast<float4*>(p0 + (long long)p * 4096) = S;
-        S.x = fmaf(f[q], S.x, add[q].x); S.y = fmaf(f[q], S.y, add[q].y);
-        S.z = fmaf(f[q], S.z, add[q].z); S.w = fmaf(f[q], S.w, add[q].w);
+      if (q0 + q < n) {
+        S.x = fmaf(d[q], S.x, f[q].x); S.y = fmaf(d[q], S.y, f[q].y);
+        S.z = fmaf(d[q], S.z, f[q].z); S.w = fmaf(d[q], S.w, f[q].w);
+        const int done = q0 + q + 1;
+        if (done % cut.sub == 0) {
+          const int p = done / cut.sub;      // parts behind the first (before the last) that this is the start of
+          *reinterpret_cast<float4*>(s0 + (long long)(reverse ? cut.parts - 1 - p : p) * 4096) = S;
+        }
       }
     }
   }
@@ -324,9 +333,7 @@ int fwd(const Args& a, cudaStream_t st) {
   constexpr int smem = (int)sizeof(FwdSmem);
   static_assert(smem <= 115712, "two CTAs of 113 KB each share an SM");
   if (int e = need_aligned_smem<la_tc_fwd_kernel<PACKED, false>>(f)) return e;
-  if (int e = need_aligned_smem<la_tc_fwd_kernel<PACKED, true>>(f)) return e;
   if (int e = allow_smem<la_tc_fwd_kernel<PACKED, false>>(f, smem)) return e;
-  if (int e = allow_smem<la_tc_fwd_kernel<PACKED, true>>(f, smem)) return e;
   const int B = t.start ? 1 : t.n_seq, T = t.start ? (int)a.w_rows : t.T, head_first = t.st == 64 && t.H > 1;
   CUtensorMap mr, mk, mv, mo;
   const void* r = a.r ? a.r : a.k;      // (the states alone: whatever r k^T is, it goes nowhere)
@@ -335,57 +342,58 @@ int fwd(const Args& a, cudaStream_t st) {
   if (int e = make_token_tensor_map(&mv, a.v, B, T, t.H, head_first)) return e;
   if (int e = make_token_tensor_map(&mo, a.o ? a.o : a.k, B, T, t.H, head_first)) return e;
   const Cut cut = cut_units(t.n_seq, t.T, t.H, false);
-  float* part_states = static_cast<float*>(a.scratch);
-  float* part_decay = part_states + (size_t)cut.n_units * cut.parts * 4096;
+  const Pieces p = pieces_at(a.scratch, cut);
   if (cut.parts > 1) {
-    {
-      ProfScope prof("linattn_tc_add_kernel", st);
-      if (int e = launch(la_tc_fwd_kernel<PACKED, true>, cut.n_units * cut.parts, NTHR, smem, st, 1, a.w, a.h0, a.n_state, (bf16*)a.o, a.ht, a.states,
-                         part_states, part_decay, mr, mk, mv, mo, t, cut, f.status)) return e;
-    }
-    if (int e = launch_chain(part_states, part_decay, a.h0, a.n_state, t, cut, false, st)) return e;
+    if (int e = launch_pieces(a, cut, mv, mk, p, false, f.status, st)) return e;
   }
   ProfScope prof("linattn_tc_fwd_kernel", st);
-  return launch(la_tc_fwd_kernel<PACKED, false>, cut.n_units * cut.parts, NTHR, smem, st, 1, a.w, a.h0, a.n_state, (bf16*)a.o, a.ht, a.states, part_states,
-                part_decay, mr, mk, mv, mo, t, cut, f.status);
+  return launch(la_tc_fwd_kernel<PACKED, false>, cut.n_units * cut.parts, NTHR, smem, st, 1, a.w, a.h0, a.n_state, (bf16*)a.o, a.ht, a.states, p.add,
+                (const float*)p.start, p.decay, (int)cut.chained(), mr, mk, mv, mo, t, cut, f.status);
 }
 
 }  // namespace
 
-int launch_tc_add(const Args& a, const Cut& cut, const CUtensorMap& map_do, const CUtensorMap& map_r, float* part_states, float* part_decay, int* status,
+int launch_pieces(const Args& a, const Cut& cut, const CUtensorMap& map_val, const CUtensorMap& map_key, const Pieces& p, bool reverse, int* status,
                   cudaStream_t st) {
-  ProfScope prof("linattn_tc_add_kernel", st);
-  constexpr int smem = (int)sizeof(FwdSmem);
   DeviceFacts f;
   if (int e = device_facts(&f)) return e;
-  const auto go = [&](auto packed) {
-    constexpr bool PACKED = decltype(packed)::value;
-    if (int e = need_aligned_smem<la_tc_fwd_kernel<PACKED, true, true>>(f)) return e;
-    if (int e = allow_smem<la_tc_fwd_kernel<PACKED, true, true>>(f, smem)) return e;
-    return launch(la_tc_fwd_kernel<PACKED, true, true>, cut.n_units * cut.parts, NTHR, smem, st, 1, a.w, (const float*)nullptr, 0, (bf16*)nullptr,
-                  (float*)nullptr, (float*)nullptr, part_states, part_decay, map_r, map_r, map_do, map_r, a.tok, cut, status);
+  constexpr int smem = (int)sizeof(AddSmem);
+  const auto go = [&](auto packed, auto rev) {
+    constexpr bool PACKED = decltype(packed)::value, REV = decltype(rev)::value;
+    if (int e = need_aligned_smem<la_tc_fwd_kernel<PACKED, true, REV>>(f)) return e;
+    if (int e = allow_smem<la_tc_fwd_kernel<PACKED, true, REV>>(f, smem)) return e;
+    ProfScope prof("linattn_tc_add_kernel", st);
+    return launch(la_tc_fwd_kernel<PACKED, true, REV>, cut.n_units * cut.adds(), NTHR, smem, st, 1, a.w, (const float*)nullptr, 0, (bf16*)nullptr,
+                  (float*)nullptr, (float*)nullptr, p.add, (const float*)nullptr, p.decay, 0, map_key, map_key, map_val, map_key, a.tok, cut, status);
   };
-  return a.tok.start ? go(std::true_type()) : go(std::false_type());
-}
-
-int launch_chain(float* part_states, const float* part_decay, const float* first, int n_first, const Tokens& t, const Cut& cut, bool reverse,
-                 cudaStream_t st) {
+  const std::true_type yes;
+  const std::false_type no;
+  if (int e = a.tok.start ? (reverse ? go(yes, yes) : go(yes, no)) : (reverse ? go(no, yes) : go(no, no))) return e;
+  if (!cut.chained()) return RWKVB200_OK;
   ProfScope prof("linattn_chain_kernel", st);
-  return launch(la_chain_kernel, cut.n_units * 4, 256, 0, st, 1, part_states, part_decay, first, n_first, t.H, cut.n_units, cut.parts, (int)reverse);
+  return launch(la_chain_kernel, cut.n_units * 4, 256, 0, st, 1, (const float*)p.add, (const float*)p.decay, p.start, reverse ? a.d_ht : a.h0,
+                reverse ? a.tok.n_seq : a.n_state, a.tok.H, cut, (int)reverse);
 }
 
-// How many stretches: as many as the device holds CTAs, where the walk over the chunks that they save is longer than the pass over keys and values and the
-// two launches that they cost (about three chunks' time).
+// How many parts and pieces: the least time by an estimate.  A chunk takes a CTA 3.9 us where two share an SM, 2.7 alone (backward 5.3, one to an SM), a chunk of
+// the pass over keys and values 2.2 where three do; another launch and what the parts start from 4 us.
 Cut cut_units(int n_seq, int max_len, int H, bool backward) {
-  const int SLOTS = backward ? 148 : 2 * 148;      // CTAs that a B200 holds
-  const int NT = (max_len + CT - 1) / CT;
-  Cut c;
-  c.n_units = n_seq * H;
-  c.parts = std::max(1, std::min(NT, SLOTS / c.n_units));
-  c.per = (NT + c.parts - 1) / c.parts;
-  if (c.parts > 1 && NT - 1.6 * c.per < 3) c.per = NT;
-  c.parts = (NT + c.per - 1) / c.per;
-  return c;
+  constexpr int SMS = 148;      // of a B200
+  const int NT = (max_len + CT - 1) / CT, units = n_seq * H, slots = backward ? SMS : 2 * SMS;
+  Cut best = {units, 1, NT, 1, NT};
+  double least = 1e30;
+  for (int parts = 1; parts <= NT && (parts == 1 || (long long)units * parts <= slots); ++parts) {
+    Cut c = {units, parts, (NT + parts - 1) / parts, 1, 0};
+    if ((NT + c.per - 1) / c.per != parts) continue;      // (the same stretches as with fewer)
+    c.sub = parts == 1 ? 1 : std::max(1, std::min(c.per, 3 * SMS / (units * (parts - 1))));
+    c.per_sub = (c.per + c.sub - 1) / c.sub;
+    c.sub = (c.per + c.per_sub - 1) / c.per_sub;
+    const long long items = (long long)units * parts;
+    const double waves = (double)((items + slots - 1) / slots);
+    const double t = waves * c.per * (backward ? 5.3 : items > SMS ? 3.9 : 2.7) + (parts > 1 ? 4 + 2.2 * c.per_sub : 0);
+    if (t < least) { least = t; best = c; }
+  }
+  return best;
 }
 
 size_t tc_states_bytes(int n_seq, int max_len, int H, bool keep) {
@@ -394,7 +402,7 @@ size_t tc_states_bytes(int n_seq, int max_len, int H, bool keep) {
 
 size_t tc_scratch_bytes(int n_seq, int max_len, int H, bool w_per_head, bool backward) {
   const Cut c = cut_units(n_seq, max_len, H, backward);
-  size_t n = c.parts > 1 ? (size_t)c.n_units * c.parts * (4096 + 1) * 4 : 0;
+  size_t n = pieces_bytes(c);
   if (backward && w_per_head) n = (n + 255) / 256 * 256 + ((size_t)n_seq * c.parts * H * 4 + 255) / 256 * 256 + (size_t)DW_PARTS * H * 8;
   return n;
 }
