@@ -3,11 +3,13 @@
 // Per group of W beams with running scores s_i (log-probabilities) and logits x_i[V]:
 //   candidate (i, t) has the score s_i + x_i[t] - log sum_u e^{x_i[u]};   the W best, ties to the lowest i V + t.
 //
-// What bounds it is reading the logits once.  The W best of a row come from its own logits in their own order, so a warp streams
-// a slice of a row and keeps, besides the running maximum and sum, the W best of what it has seen, sorted, one to a lane.  After the first
-// tiles hardly any element passes the W-th best (W ln(n / W) of n), so that list costs a comparison per element and a shuffle of a few
-// instructions now and then.  One cluster of CTAs works on a group; its warps' lists and sums meet in the shared memory of the first CTA, where
-// the normalisers are put together and candidates compared in float64: a sum of two float32 would tie where the scores do not.
+// What bounds it is reading the logits once.  The W best of a row come from its own logits in their own order.  A warp streams a slice of a row and
+// keeps, for each lane, the running maximum, the tile it is in, the largest of the other tiles and the running sum: some 150 instructions for 512 tokens, where
+// sorted lists kept on the way took three times that in time.  The W-th largest of the lanes' maxima is at most the W-th best of the row, so only the lanes that
+// reach it have any of the W best: a few of the row's lanes, of which 16 tokens each (all, where another tile reaches it, too) are read once more, from L2, and
+// offered to a list.  One cluster of CTAs works on a group; its warps' lists and sums meet in the shared memory of the first CTA, where the normalisers are put
+// together and candidates compared in float64: a sum of two float32 would tie where the scores do not.
+// What runs once is kept short in code: it is fetched while everyone waits for it.
 //
 // A beam that has finished goes on with `eos` alone, at the score it has; its logits are not read.  NaN and +inf logits count as -inf (never
 // generated), a NaN score as -inf.  Where fewer than W candidates are possible the rest are impossible ones, score -inf, lowest
@@ -15,6 +17,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "tc.cuh"
@@ -68,59 +71,52 @@ __device__ __forceinline__ void offer(Best<F, I>& b, F x, I j, int W, int lane) 
   offer(b, wv, wi, x, j, W, lane);
 }
 
-template <typename T> struct Vec { static constexpr int N = 16 / (int)sizeof(T); };
-// 16 bytes of logits as floats, those that are NaN or +inf as -inf
+// Logits as floats, those that are NaN or +inf as -inf.
 __device__ __forceinline__ float clean(float x) { return x <= FLT_MAX ? x : NEG; }
-__device__ __forceinline__ void unpack(const uint4& u, float* x, const float*) {
-  x[0] = __uint_as_float(u.x); x[1] = __uint_as_float(u.y); x[2] = __uint_as_float(u.z); x[3] = __uint_as_float(u.w);
-}
-__device__ __forceinline__ void unpack(const uint4& u, float* x, const __nv_bfloat16*) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) { x[2 * i] = __uint_as_float(w[i] << 16); x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-}
-__device__ __forceinline__ void unpack(const uint4& u, float* x, const __half*) {
-  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-    x[2 * i] = f.x; x[2 * i + 1] = f.y;
-  }
-}
 
-// Piece p of a row, its elements p N .. p N + N - 1, whatever the row's alignment: every piece is the same elements in every row, so that
-// equal rows have equal sums to the last bit.  A row that does not start on 16 bytes (`shift` bytes behind it) has its pieces cut out of two
-// aligned ones, the second of which the next lane reads as well (it comes from L1); where these reach over the ends of the row, or the row ends in the
-// piece, elements are read one by one.  Elements behind the end are -inf.
+// A tile: 512 tokens of a row, 16 to a lane, in words of 4 bytes that lie next to each other across the lanes: nothing but the element's own alignment is asked
+// of a row (and not even a word's of 16-bit rows of odd length), and every tile is the same tokens of the same lanes in every row, so that equal rows have
+// equal sums to the last bit.
+constexpr int TILE = 512;
 template <typename T>
-__device__ __forceinline__ void fetch(const T* x, int p, int V, int shift, uint4 (&u)[2]) {
-  constexpr int N = Vec<T>::N;
-  const int e = p * N - shift / (int)sizeof(T);      // the first element of the aligned piece
-  if (shift == 0 ? e + N <= V : e >= 0 && e + 2 * N <= V) {
-    u[0] = __ldg(reinterpret_cast<const uint4*>(x + e));
-    if (shift) u[1] = __ldg(reinterpret_cast<const uint4*>(x + e) + 1);
-  } else {      // (put where align() finds it)
-    __align__(16) T t[2 * N];
+struct Tile {
+  static constexpr int PER = 4 / (int)sizeof(T), N = 16 / PER;      // elements of a word, words of a lane
+  uint32_t w[N];
+  // the token of element i of a lane
+  static __device__ __forceinline__ int token(int base, int lane, int i) { return base + (i / PER) * (32 * PER) + PER * lane + i % PER; }
+  __device__ __forceinline__ void load(const T* x, int base, int V, int lane, bool words) {
+    const bool whole = base + TILE <= V;
 #pragma unroll
-    for (int i = 0; i < 2 * N; ++i) t[i] = e + i >= p * N && e + i < min(V, p * N + N) ? x[e + i] : from_f32<T>(NEG);
-    u[0] = *reinterpret_cast<const uint4*>(t);
-    u[1] = *reinterpret_cast<const uint4*>(t + N);
+    for (int q = 0; q < N; ++q) {
+      const int t = token(base, lane, q * PER);
+      if constexpr (PER == 1) {
+        w[q] = whole || t < V ? __ldg(reinterpret_cast<const uint32_t*>(x) + t) : 0xff800000u;
+      } else {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+        constexpr uint32_t none = std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;      // -inf
+        if (words && (whole || t + 1 < V)) {
+          w[q] = __ldg(reinterpret_cast<const uint32_t*>(h + t));
+        } else {
+          const uint32_t lo = t < V ? __ldg(h + t) : none, hi = t + 1 < V ? __ldg(h + t + 1) : none;
+          w[q] = lo | hi << 16;
+        }
+      }
+    }
   }
-}
-__device__ __forceinline__ void align(uint4 (&u)[2], int shift) {      // (a warp has one row: no lane takes another way)
-  const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
-  auto cut = [&](int i) {
-    if (shift & 2) u[0] = make_uint4(__funnelshift_r(w[i], w[i + 1], 16), __funnelshift_r(w[i + 1], w[i + 2], 16),
-                                     __funnelshift_r(w[i + 2], w[i + 3], 16), __funnelshift_r(w[i + 3], w[i + 4], 16));
-    else u[0] = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-  };
-  switch (shift >> 2) {
-    case 1: cut(1); break;
-    case 2: cut(2); break;
-    case 3: cut(3); break;
-    default: cut(0);
+  __device__ __forceinline__ void values(float (&f)[16]) const {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      if constexpr (PER == 1) {
+        f[q] = clean(__uint_as_float(w[q]));
+      } else if constexpr (std::is_same<T, __half>::value) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[q]));
+        f[2 * q] = clean(v.x); f[2 * q + 1] = clean(v.y);
+      } else {
+        f[2 * q] = clean(__uint_as_float(w[q] << 16)); f[2 * q + 1] = clean(__uint_as_float(w[q] & 0xffff0000u));
+      }
+    }
   }
-}
+};
 
 // Running maximum and sum of a lane, in float32: a lane adds a few hundred terms that are at most one.
 struct Sum {
@@ -138,11 +134,36 @@ struct Sum {
 
 struct Smem {
   float m[MAXC * NWARP], s[MAXC * NWARP];          // in the first CTA: of every warp of the cluster
-  float val[MAXC * NWARP][MAXW];
-  int tok[MAXC * NWARP][MAXW];
+  float val[MAXC * NWARP * MAXW];                  // [warp][W]
+  int tok[MAXC * NWARP * MAXW];
   double top[MAXW], shift[MAXW];                   // of a row: the maximum; s_i - log (sum relative to it)
-  GroupBest best[NWARP][MAXW];
+  RowBest best[MAXW][MAXW];                        // of a row: its W best
+  float top_lanes[NWARP][MAXW];                    // of this CTA's warps, the W largest of the lanes' maxima
 };
+// The cluster's barrier, for threads that may come to it apart: what goes before it here are loops and choices of single lanes.
+__device__ __forceinline__ void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+  __syncwarp();
+}
+// the lanes' x in descending order
+__device__ __noinline__ float sort_lanes(float x) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll 1
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll 1
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const float y = __shfl_xor_sync(0xffffffffu, x, j);
+      const bool larger = ((lane & j) == 0) == ((lane & k) == 0);      // (descending as a whole: lane & 32 is 0)
+      x = larger ? fmaxf(x, y) : fminf(x, y);
+    }
+  return x;
+}
+// the n-th largest of the lanes' x, in every lane
+__device__ __forceinline__ float nth_largest(float x, int n) { return __shfl_sync(0xffffffffu, sort_lanes(x), n - 1); }
 
 template <typename T>
 __global__ void __launch_bounds__(NWARP * 32, 2)
@@ -157,41 +178,58 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
   const int all = rank * NWARP + warp, row = all / per_row, part = all % per_row;
   earlier_kernels_done();
   later_kernels_may_start();
-  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // (the first CTA has to be there before it is written to)
+  cluster_arrive();      // (the first CTA has to be there before it is written to)
   RowBest best;      // of this warp's slice
   Sum sum;
-  const bool works = row < W;
-  const bool done = works && finished && finished[(long long)g * W + row];
-  if (works && !done) {
-    constexpr int N = Vec<T>::N, U = 16 / N;      // 16 elements of a lane at a time, in pieces of 16 bytes
-    const T* x = logits + g * stride_g + row * stride_w;
-    const int shift = (int)(reinterpret_cast<uintptr_t>(x) & 15);
-    const int n_piece = (V + N - 1) / N;
-    const int lo = (int)((long long)n_piece * part / per_row), hi = (int)((long long)n_piece * (part + 1) / per_row);
-    float wv = NEG;      // the W-th best
-    int wi = RowBest::NONE;
-    for (int p = lo + lane; p - lane < hi; p += 32 * U) {
-      uint4 u4[U][2];
-#pragma unroll
-      for (int u = 0; u < U; ++u) fetch(x, p + 32 * u < hi ? p + 32 * u : n_piece, V, shift, u4[u]);
+  const bool works = row < W && !(finished && finished[(long long)g * W + row]);
+  const T* x = logits + g * stride_g + row * stride_w;
+  const int n_tile = (V + TILE - 1) / TILE;
+  const int lo = works ? (int)((long long)n_tile * part / per_row) : 0, hi = works ? (int)((long long)n_tile * (part + 1) / per_row) : 0;
+  float other = NEG;      // the largest of a lane's tokens outside the tile with its maximum
+  int at = lo;            // that tile
+  if (lo < hi) {
+    const bool words = (reinterpret_cast<uintptr_t>(x) & 3) == 0;
+    Tile<T> next[2];      // the next tiles are on their way while one is looked at
+    next[0].load(x, lo * TILE, V, lane, words);
+    if (lo + 1 < hi) next[1].load(x, (lo + 1) * TILE, V, lane, words);
+#pragma unroll 1
+    for (int t = lo; t < hi; ++t) {
+      const Tile<T> tile = next[0];
+      next[0] = next[1];
+      if (t + 2 < hi) next[1].load(x, (t + 2) * TILE, V, lane, words);
       float f[16];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        align(u4[u], shift);
-        unpack(u4[u][0], f + u * N, (const T*)nullptr);
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) f[i] = clean(f[i]);
+      tile.values(f);
       float top = f[0];
 #pragma unroll
       for (int i = 1; i < 16; ++i) top = fmaxf(top, f[i]);
+      other = fmaxf(other, fminf(top, sum.m));
+      if (top > sum.m) at = t;
       sum.add(f, top);
-      if (__any_sync(0xffffffffu, before(top, p * N, wv, wi))) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int q = p + 32 * (i / N), j = q * N + i % N;
-          offer(best, wv, wi, f[i], q < hi && j < V ? j : RowBest::NONE, W, lane);
-        }
+    }
+  }
+  const float sorted = sort_lanes(sum.m);
+  if (lane < W) sm.top_lanes[warp][lane] = sorted;
+  __syncthreads();
+  if (lo < hi) {
+    // what the row's W best are at least, as far as this CTA's warps know: of the warps' W largest, folded onto 32 lanes, the W-th largest
+    const int w0 = max(0, warp - part), w1 = min(NWARP, warp - part + per_row);      // (a row's warps that lie in this CTA)
+    float most = NEG;
+    for (int e = lane; e < (w1 - w0) * W; e += 32) most = fmaxf(most, sm.top_lanes[w0 + e / W][e % W]);
+    const float least = nth_largest(most, W);      // (-inf where few tokens are possible: then the impossible ones count, too)
+    float wv = NEG;
+    int wi = RowBest::NONE;
+    uint32_t lanes = __ballot_sync(0xffffffffu, sum.m >= least);
+    while (lanes) {
+      const int l = __ffs(lanes) - 1;
+      lanes &= lanes - 1;
+      const bool all = __shfl_sync(0xffffffffu, other, l) >= least;
+      const int t0 = all ? lo : __shfl_sync(0xffffffffu, at, l), n = all ? (hi - lo) * 16 : 16;
+#pragma unroll 1
+      for (int e = lane; e - lane < n; e += 32) {
+        const int j = Tile<T>::token((t0 + (e >> 4)) * TILE, l, e & 15);
+        const bool have = e < n && j < V;
+        const float f = have ? clean(to_f32(x[j])) : NEG;
+        offer(best, wv, wi, f, have && f >= least ? j : RowBest::NONE, W, lane);
       }
     }
   }
@@ -202,58 +240,90 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
   float s = sum.m == NEG ? 0.f : sum.s * tc::ex2((sum.m - m) * tc::LOG2E);
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+  cluster_wait();
   const uint32_t home = tc::cluster_addr(tc::smem_u32(&sm), 0);
   auto put = [&](const void* p, int bits) { tc::store_cluster(home + (tc::smem_u32(p) - tc::smem_u32(&sm)), bits); };
   if (lane == 0) { put(&sm.m[all], __float_as_int(m)); put(&sm.s[all], __float_as_int(s)); }
-  if (lane < W) { put(&sm.val[all][lane], __float_as_int(best.v)); put(&sm.tok[all][lane], best.i == RowBest::NONE ? -1 : best.i); }
-  tc::cluster_sync();
+  if (lane < W) { put(&sm.val[all * W + lane], __float_as_int(best.v)); put(&sm.tok[all * W + lane], best.i); }
+  cluster_arrive();
+  cluster_wait();
   if (rank) return;
 
-  for (int i = warp; i < W; i += NWARP) {
+  // The rows' own W best, and their normalisers: two warps to a row where there are enough.
+  const bool apart = 2 * W <= NWARP;
+  for (int i = apart ? warp >> 1 : warp; i < W; i += NWARP) {
+    const bool over = finished && finished[(long long)g * W + i];
     const float score = scores[(long long)g * W + i];
-    double mm = NEG, ss = 0.0;
-    for (int q = lane; q < per_row; q += 32) mm = fmax(mm, (double)sm.m[i * per_row + q]);
+    if (!apart || (warp & 1)) {
+      double mm = NEG, ss = 0.0;
+      for (int q = lane; q < per_row; q += 32) mm = fmax(mm, (double)sm.m[i * per_row + q]);
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) mm = fmax(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-    for (int q = lane; q < per_row; q += 32) {
-      const float mq = sm.m[i * per_row + q];
-      if (mq != NEG) ss += (double)sm.s[i * per_row + q] * exp((double)mq - mm);
-    }
-#pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-    // (a row without a possible token: every candidate is -inf)
-    if (lane == 0) {      // (the maximum apart: only differences of logits count, however large these are)
-      sm.top[i] = mm;
-      sm.shift[i] = score != score ? (double)NEG : ss > 0.0 ? (double)score - log(ss) : (double)NEG;
-    }
-  }
-  __syncthreads();
-  GroupBest b;
-  auto offer_row = [&](int i, float x, long long t) {      // t < 0: nothing
-    const double sc = x == NEG ? (double)NEG : sm.shift[i] + ((double)x - sm.top[i]);
-    offer(b, t < 0 ? (double)NEG : sc, t < 0 ? GroupBest::NONE : (long long)i * V + t, W, lane);
-  };
-  for (int q = warp; q < W * per_row; q += NWARP) {
-    const int i = q / per_row;
-    if (finished && finished[(long long)g * W + i]) {
-      if (q % per_row == 0) {      // eos at the beam's score, and (impossible) tokens from the first one on
-        const float score = scores[(long long)g * W + i];
-        long long t = lane == 0 ? eos : lane - 1 < eos ? lane - 1 : lane;
-        if (t >= V) t = -1;
-        offer(b, lane == 0 && score == score ? (double)score : (double)NEG, t < 0 ? GroupBest::NONE : (long long)i * V + t, W, lane);
-        if (W == 32) offer(b, (double)NEG, lane == 0 && eos >= 32 && 31 < V ? (long long)i * V + 31 : GroupBest::NONE, W, lane);
+      for (int d = 16; d >= 1; d >>= 1) mm = fmax(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+      for (int q = lane; q < per_row; q += 32) {
+        const float mq = sm.m[i * per_row + q];
+        if (mq != NEG) ss += (double)(sm.s[i * per_row + q] * tc::ex2((mq - (float)mm) * tc::LOG2E));
       }
-      continue;
+#pragma unroll
+      for (int d = 16; d >= 1; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+      // (a row without a possible token: every candidate is -inf)
+      if (lane == 0) {      // (the maximum apart: only differences of logits count, however large these are)
+        sm.top[i] = mm;
+        sm.shift[i] = score != score ? (double)NEG : ss > 0.0 ? (double)score - log(ss) : (double)NEG;
+      }
     }
-    offer_row(i, lane < W ? sm.val[q][lane] : NEG, lane < W ? sm.tok[q][lane] : -1);
+    if (!apart || !(warp & 1)) {
+      RowBest b;
+      if (!over) {
+        const int n = per_row * W;      // entries of the warps' lists, some of them empty
+        float most = NEG;
+        for (int e = lane; e < n; e += 32) most = fmaxf(most, sm.val[i * n + e]);
+        const float least = nth_largest(most, W);
+#pragma unroll 1
+        for (int e = lane; e - lane < n; e += 32) {
+          const float v = e < n ? sm.val[i * n + e] : NEG;
+          offer(b, v, e < n && v >= least ? sm.tok[i * n + e] : RowBest::NONE, W, lane);
+        }
+      } else {      // (impossible) tokens from the first one on, but eos
+        const int t = lane < (int)eos ? lane : lane + 1;
+        b.i = t < V ? t : RowBest::NONE;
+      }
+      sm.best[i][lane] = b;
+    }
   }
-  sm.best[warp][lane] = b;
   __syncthreads();
   if (warp) return;
-  for (int q = 1; q < NWARP; ++q) {
-    const GroupBest c = sm.best[q][lane];
-    offer(b, lane < W ? c.v : (double)NEG, lane < W ? c.i : GroupBest::NONE, W, lane);
+  GroupBest b;
+  const auto entry = [&](int e, double& score) -> long long {      // one of the rows' W best
+    score = NEG;
+    const bool eos_of = e >= W * W;
+    const int i = eos_of ? e - W * W : e / W, at = e - i * W;
+    if (i >= W) return GroupBest::NONE;
+    const bool over = finished && finished[(long long)g * W + i];
+    if (eos_of) {
+      const float s = over ? scores[(long long)g * W + i] : NEG;
+      if (s == s) score = s;
+      return over ? (long long)i * V + eos : GroupBest::NONE;
+    }
+    RowBest c = sm.best[i][at];
+    if (!over) {
+      if (sm.shift[i] == (double)NEG) c.i = at < V ? at : RowBest::NONE;      // a beam that is impossible: all its tokens are, the first ones first
+      else if (c.v != NEG) score = sm.shift[i] + ((double)c.v - sm.top[i]);
+    }
+    return c.i == RowBest::NONE ? GroupBest::NONE : (long long)i * V + c.i;
+  };
+  // (and, behind the rows', the finished beams' eos)
+  float most = NEG;
+  for (int e = lane; e < W * W + W; e += 32) {
+    double score;
+    entry(e, score);
+    most = fmaxf(most, (float)score);      // (rounding keeps the order)
+  }
+  const float least = nth_largest(most, W);
+#pragma unroll 1
+  for (int e = lane; e - lane < W * W + W; e += 32) {
+    double score;
+    const long long j = entry(e, score);
+    offer(b, score, (float)score >= least ? j : GroupBest::NONE, W, lane);
   }
   if (lane < W) {
     const long long at = (long long)g * W + lane, parent = b.i / V, t = b.i - parent * V;
@@ -275,7 +345,7 @@ int select(const void* logits, long long sg, long long sw, const float* scores, 
   // beams, and no more CTAs than there are pieces of a few tiles to work on
   int c = MAXC;
   while (c > 1 && (long long)G * c > 2 * f.sms) c >>= 1;
-  while (c > 1 && (long long)W * V < (long long)c * NWARP * 256) c >>= 1;
+  while (c > 1 && (long long)W * V <= (long long)(c >> 1) * NWARP * TILE) c >>= 1;
   while (c * NWARP < W) c <<= 1;
   return launch(beam_select_kernel<T>, dim3(G, c), NWARP * 32, smem, st, c == 1 ? 1 : c, (const T*)logits, sg, sw, scores, finished, eos, scores_out,
                 parents, tokens, finished_out, W, V);

@@ -81,6 +81,18 @@ def test_masked_tokens_dead_beams_and_bad_numbers(dtype):
     check(nothing, torch.tensor([[math.nan, -1.0, -2.0]]), torch.tensor([[True, False, True]]), 0)
 
 
+@pytest.mark.parametrize("W,V", [(4, 600), (3, 2), (32, 5), (32, 4000)])
+def test_dead_beams(W, V):
+    """Beams that do not exist (score -inf) go on with nothing: their candidates come last, the first tokens first, whatever their logits."""
+    logits, scores, g = inputs(3, W, V, torch.float32, 9)
+    scores[0] = -math.inf
+    scores[1, 1:] = -math.inf
+    scores[2, 0] = -math.inf
+    logits[2, 1, 1:] = -math.inf
+    check(logits, scores)
+    check(logits, scores, torch.rand(3, W, generator=g) < 0.5, V - 1)
+
+
 @pytest.mark.parametrize("eos", [0, 3, 31, 32, 40])
 def test_all_beams_finished(eos):
     G, W, V = 2, 32, 41
