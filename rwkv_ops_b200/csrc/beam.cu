@@ -132,14 +132,23 @@ struct Sum {
   }
 };
 
+// A token and its logit as one number, larger is better: the logit's bits in the order of the numbers, then the complement of the token.  0: none.
+typedef unsigned long long Key;
+__device__ __forceinline__ uint32_t key_hi(float v) { const uint32_t u = __float_as_uint(v); return u >> 31 ? ~u : u | 0x80000000u; }
+__device__ __forceinline__ float key_logit(Key k) { const uint32_t u = (uint32_t)(k >> 32); return __uint_as_float(u >> 31 ? u & 0x7fffffffu : ~u); }
+__device__ __forceinline__ int key_token(Key k) { return (int)~(uint32_t)k; }
+
 struct Smem {
-  float m[MAXC * NWARP], s[MAXC * NWARP];          // in the first CTA: of every warp of the cluster
-  float val[MAXC * NWARP * MAXW];                  // [warp][W]
-  int tok[MAXC * NWARP * MAXW];
+  union {
+    Key key[MAXC * NWARP * MAXW];                  // in the first CTA: of every warp of the cluster, the W best of its slice [warp][W]
+    struct { double score[MAXW * MAXW + MAXW]; long long at[MAXW * MAXW + MAXW]; } last;      // then the group's candidates
+  };
+  Key best[MAXW][MAXW];                            // of a row: its W best
+  float m[MAXC * NWARP], s[MAXC * NWARP];          // of every warp of the cluster
   double top[MAXW], shift[MAXW];                   // of a row: the maximum; s_i - log (sum relative to it)
-  RowBest best[MAXW][MAXW];                        // of a row: its W best
   float top_lanes[NWARP][MAXW];                    // of this CTA's warps, the W largest of the lanes' maxima
 };
+static_assert(sizeof(Smem) <= 48 * 1024, "");
 // The cluster's barrier, for threads that may come to it apart: what goes before it here are loops and choices of single lanes.
 __device__ __forceinline__ void cluster_arrive() {
   __syncwarp();
@@ -150,11 +159,10 @@ __device__ __forceinline__ void cluster_wait() {
   __syncwarp();
 }
 // the lanes' x in descending order
-__device__ __noinline__ float sort_lanes(float x) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll 1
+__device__ __forceinline__ float sort_lanes(float x, int lane) {
+#pragma unroll
   for (int k = 2; k <= 32; k <<= 1)
-#pragma unroll 1
+#pragma unroll
     for (int j = k >> 1; j > 0; j >>= 1) {
       const float y = __shfl_xor_sync(0xffffffffu, x, j);
       const bool larger = ((lane & j) == 0) == ((lane & k) == 0);      // (descending as a whole: lane & 32 is 0)
@@ -163,7 +171,7 @@ __device__ __noinline__ float sort_lanes(float x) {
   return x;
 }
 // the n-th largest of the lanes' x, in every lane
-__device__ __forceinline__ float nth_largest(float x, int n) { return __shfl_sync(0xffffffffu, sort_lanes(x), n - 1); }
+__device__ __forceinline__ float nth_largest(float x, int n, int lane) { return __shfl_sync(0xffffffffu, sort_lanes(x, lane), n - 1); }
 
 template <typename T>
 __global__ void __launch_bounds__(NWARP * 32, 2)
@@ -207,7 +215,7 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
       sum.add(f, top);
     }
   }
-  const float sorted = sort_lanes(sum.m);
+  const float sorted = sort_lanes(sum.m, lane);
   if (lane < W) sm.top_lanes[warp][lane] = sorted;
   __syncthreads();
   if (lo < hi) {
@@ -215,22 +223,27 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
     const int w0 = max(0, warp - part), w1 = min(NWARP, warp - part + per_row);      // (a row's warps that lie in this CTA)
     float most = NEG;
     for (int e = lane; e < (w1 - w0) * W; e += 32) most = fmaxf(most, sm.top_lanes[w0 + e / W][e % W]);
-    const float least = nth_largest(most, W);      // (-inf where few tokens are possible: then the impossible ones count, too)
+    const float least = nth_largest(most, W, lane);      // (-inf where few tokens are possible: then the impossible ones count, too)
     float wv = NEG;
     int wi = RowBest::NONE;
-    uint32_t lanes = __ballot_sync(0xffffffffu, sum.m >= least);
-    while (lanes) {
-      const int l = __ffs(lanes) - 1;
-      lanes &= lanes - 1;
-      const bool all = __shfl_sync(0xffffffffu, other, l) >= least;
-      const int t0 = all ? lo : __shfl_sync(0xffffffffu, at, l), n = all ? (hi - lo) * 16 : 16;
-#pragma unroll 1
-      for (int e = lane; e - lane < n; e += 32) {
-        const int j = Tile<T>::token((t0 + (e >> 4)) * TILE, l, e & 15);
-        const bool have = e < n && j < V;
-        const float f = have ? clean(to_f32(x[j])) : NEG;
-        offer(best, wv, wi, f, have && f >= least ? j : RowBest::NONE, W, lane);
-      }
+    const uint32_t lanes = __ballot_sync(0xffffffffu, sum.m >= least), whole = lanes & __ballot_sync(0xffffffffu, other >= least);
+    const auto look = [&](int j, bool have) {
+      have = have && j < V;
+      const float f = have ? clean(to_f32(x[j])) : NEG;
+      offer(best, wv, wi, f, have && f >= least ? j : RowBest::NONE, W, lane);
+    };
+    for (uint32_t left = lanes & ~whole; left;) {      // one tile of two lanes' tokens at a time
+      const int l0 = __ffs(left) - 1;
+      left &= left - 1;
+      const int l1 = left ? __ffs(left) - 1 : l0;
+      const bool two = left != 0;
+      left &= left - 1;
+      const int l = lane < 16 ? l0 : l1, t0 = __shfl_sync(0xffffffffu, at, l);
+      look(Tile<T>::token(t0 * TILE, l, lane & 15), lane < 16 || two);
+    }
+    for (uint32_t left = whole; left; left &= left - 1) {      // all tiles of a lane's
+      const int l = __ffs(left) - 1, n = (hi - lo) * 16;
+      for (int e = lane; e - lane < n; e += 32) look(Tile<T>::token((lo + (e >> 4)) * TILE, l, e & 15), e < n);
     }
   }
   // the warp's sum, relative to its maximum
@@ -242,95 +255,91 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
   for (int d = 16; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   cluster_wait();
   const uint32_t home = tc::cluster_addr(tc::smem_u32(&sm), 0);
-  auto put = [&](const void* p, int bits) { tc::store_cluster(home + (tc::smem_u32(p) - tc::smem_u32(&sm)), bits); };
+  auto put = [&](const void* p, int bits) {      // a word to the first CTA
+    tc::store_cluster(home + (tc::smem_u32(p) - tc::smem_u32(&sm)), bits); };
   if (lane == 0) { put(&sm.m[all], __float_as_int(m)); put(&sm.s[all], __float_as_int(s)); }
-  if (lane < W) { put(&sm.val[all * W + lane], __float_as_int(best.v)); put(&sm.tok[all * W + lane], best.i); }
+  if (lane < W) {
+    const uint32_t* k = reinterpret_cast<const uint32_t*>(&sm.key[all * W + lane]);
+    const bool any = best.i != RowBest::NONE;
+    put(k, any ? (int)~(uint32_t)best.i : 0);
+    put(k + 1, any ? (int)key_hi(best.v + 0.f) : 0);      // (zeros of either sign are equal)
+  }
   cluster_arrive();
   cluster_wait();
   if (rank) return;
 
-  // The rows' own W best, and their normalisers: two warps to a row where there are enough.
-  const bool apart = 2 * W <= NWARP;
-  for (int i = apart ? warp >> 1 : warp; i < W; i += NWARP) {
-    const bool over = finished && finished[(long long)g * W + i];
+  // The rows' normalisers, a warp to a row, and their W best: the place of a candidate is the number of those before it, counted by a thread.
+  for (int i = threadIdx.x; i < W * MAXW; i += NWARP * 32) sm.best[i / MAXW][i % MAXW] = 0;
+  for (int i = warp; i < W; i += NWARP) {
     const float score = scores[(long long)g * W + i];
-    if (!apart || (warp & 1)) {
-      double mm = NEG, ss = 0.0;
-      for (int q = lane; q < per_row; q += 32) mm = fmax(mm, (double)sm.m[i * per_row + q]);
+    float mm = NEG;
+    for (int q = lane; q < per_row; q += 32) mm = fmaxf(mm, sm.m[i * per_row + q]);
 #pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) mm = fmax(mm, __shfl_xor_sync(0xffffffffu, mm, d));
-      for (int q = lane; q < per_row; q += 32) {
-        const float mq = sm.m[i * per_row + q];
-        if (mq != NEG) ss += (double)(sm.s[i * per_row + q] * tc::ex2((mq - (float)mm) * tc::LOG2E));
-      }
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-      // (a row without a possible token: every candidate is -inf)
-      if (lane == 0) {      // (the maximum apart: only differences of logits count, however large these are)
-        sm.top[i] = mm;
-        sm.shift[i] = score != score ? (double)NEG : ss > 0.0 ? (double)score - log(ss) : (double)NEG;
-      }
+    for (int d = 16; d >= 1; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
+    double ss = 0.0;
+    for (int q = lane; q < per_row; q += 32) {
+      const float mq = sm.m[i * per_row + q];
+      if (mq != NEG) ss += (double)(sm.s[i * per_row + q] * tc::ex2((mq - mm) * tc::LOG2E));
     }
-    if (!apart || !(warp & 1)) {
-      RowBest b;
-      if (!over) {
-        const int n = per_row * W;      // entries of the warps' lists, some of them empty
-        float most = NEG;
-        for (int e = lane; e < n; e += 32) most = fmaxf(most, sm.val[i * n + e]);
-        const float least = nth_largest(most, W);
-#pragma unroll 1
-        for (int e = lane; e - lane < n; e += 32) {
-          const float v = e < n ? sm.val[i * n + e] : NEG;
-          offer(b, v, e < n && v >= least ? sm.tok[i * n + e] : RowBest::NONE, W, lane);
-        }
-      } else {      // (impossible) tokens from the first one on, but eos
-        const int t = lane < (int)eos ? lane : lane + 1;
-        b.i = t < V ? t : RowBest::NONE;
-      }
-      sm.best[i][lane] = b;
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+    // (a row without a possible token: every candidate is -inf)
+    if (lane == 0) {      // (the maximum apart: only differences of logits count, however large these are)
+      sm.top[i] = mm;
+      sm.shift[i] = score != score ? (double)NEG : ss > 0.0 ? (double)score - log(ss) : (double)NEG;
     }
   }
   __syncthreads();
-  if (warp) return;
-  GroupBest b;
-  const auto entry = [&](int e, double& score) -> long long {      // one of the rows' W best
-    score = NEG;
-    const bool eos_of = e >= W * W;
-    const int i = eos_of ? e - W * W : e / W, at = e - i * W;
-    if (i >= W) return GroupBest::NONE;
+  const int n_key = per_row * W;      // of a row
+  for (int e = threadIdx.x; e < W * n_key; e += NWARP * 32) {
+    const Key mine = sm.key[e];
+    if (!mine) continue;
+    const Key* k = sm.key + e / n_key * n_key;
+    int place = 0;
+#pragma unroll 8
+    for (int q = 0; q < n_key; ++q) place += k[q] > mine;
+    if (place < W) sm.best[e / n_key][place] = mine;
+  }
+  __syncthreads();
+  // The group's candidates: the rows' W best and, behind them, the finished beams' eos.
+  const int n_last = W * W + W;
+  for (int e = threadIdx.x; e < n_last; e += NWARP * 32) {
+    const int i = e < W * W ? e / W : e - W * W, at = e - i * W;
     const bool over = finished && finished[(long long)g * W + i];
-    if (eos_of) {
-      const float s = over ? scores[(long long)g * W + i] : NEG;
-      if (s == s) score = s;
-      return over ? (long long)i * V + eos : GroupBest::NONE;
+    double score = NEG;
+    int t = -1;      // (none)
+    if (e >= W * W) {
+      if (over) {
+        const float s = scores[(long long)g * W + i];
+        if (s == s) score = s;
+        t = (int)eos;
+      }
+    } else if (over) {                            // impossible tokens from the first one on, but eos
+      t = at < (int)eos ? at : at + 1;
+    } else if (sm.shift[i] == (double)NEG) {      // a beam that is impossible: all its tokens are, the first ones first
+      t = at;
+    } else if (const Key k = sm.best[i][at]) {
+      t = key_token(k);
+      if (key_logit(k) != NEG) score = sm.shift[i] + ((double)key_logit(k) - sm.top[i]);
     }
-    RowBest c = sm.best[i][at];
-    if (!over) {
-      if (sm.shift[i] == (double)NEG) c.i = at < V ? at : RowBest::NONE;      // a beam that is impossible: all its tokens are, the first ones first
-      else if (c.v != NEG) score = sm.shift[i] + ((double)c.v - sm.top[i]);
+    sm.last.score[e] = score;
+    sm.last.at[e] = t < 0 || t >= V ? GroupBest::NONE : (long long)i * V + t;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < n_last; e += NWARP * 32) {
+    const double score = sm.last.score[e];
+    const long long j = sm.last.at[e];
+    if (j == GroupBest::NONE) continue;
+    int place = 0;
+#pragma unroll 4
+    for (int q = 0; q < n_last; ++q) place += before(sm.last.score[q], sm.last.at[q], score, j);
+    if (place < W) {
+      const long long at = (long long)g * W + place, parent = j / V, t = j - parent * V;
+      scores_out[at] = (float)score;
+      parents[at] = parent;
+      tokens[at] = t;
+      if (finished_out) finished_out[at] = (finished && finished[(long long)g * W + parent]) || t == eos;
     }
-    return c.i == RowBest::NONE ? GroupBest::NONE : (long long)i * V + c.i;
-  };
-  // (and, behind the rows', the finished beams' eos)
-  float most = NEG;
-  for (int e = lane; e < W * W + W; e += 32) {
-    double score;
-    entry(e, score);
-    most = fmaxf(most, (float)score);      // (rounding keeps the order)
-  }
-  const float least = nth_largest(most, W);
-#pragma unroll 1
-  for (int e = lane; e - lane < W * W + W; e += 32) {
-    double score;
-    const long long j = entry(e, score);
-    offer(b, score, (float)score >= least ? j : GroupBest::NONE, W, lane);
-  }
-  if (lane < W) {
-    const long long at = (long long)g * W + lane, parent = b.i / V, t = b.i - parent * V;
-    scores_out[at] = (float)b.v;
-    parents[at] = parent;
-    tokens[at] = t;
-    if (finished_out) finished_out[at] = (finished && finished[(long long)g * W + parent]) || t == eos;
   }
 }
 

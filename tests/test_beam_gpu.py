@@ -56,6 +56,8 @@ def test_ties_go_to_the_lowest(dtype, W):
     rising = torch.arange(V).div(100, rounding_mode="floor").to(dtype).expand(2, W, V).contiguous()
     check(rising, scores)
     check(rising.flip(-1).contiguous(), scores)
+    signs = torch.randint(0, 2, (2, 1, V), generator=g).expand(2, W, V).contiguous()
+    check(torch.where(signs == 0, 0.0, -0.0).to(dtype), scores)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
