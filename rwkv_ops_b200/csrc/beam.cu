@@ -227,23 +227,40 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
     float wv = NEG;
     int wi = RowBest::NONE;
     const uint32_t lanes = __ballot_sync(0xffffffffu, sum.m >= least), whole = lanes & __ballot_sync(0xffffffffu, other >= least);
-    const auto look = [&](int j, bool have) {
-      have = have && j < V;
-      const float f = have ? clean(to_f32(x[j])) : NEG;
-      offer(best, wv, wi, f, have && f >= least ? j : RowBest::NONE, W, lane);
+    // (all that is going to be looked at next is asked for before the first of it is: the way to L2 is what this takes)
+    constexpr int AHEAD = 4;
+    float f[AHEAD];
+    int token[AHEAD];
+    const auto ask = [&](int q, int j, bool have) {
+      token[q] = have && j < V ? j : RowBest::NONE;
+      f[q] = token[q] != RowBest::NONE ? clean(to_f32(x[j])) : NEG;
     };
-    for (uint32_t left = lanes & ~whole; left;) {      // one tile of two lanes' tokens at a time
-      const int l0 = __ffs(left) - 1;
-      left &= left - 1;
-      const int l1 = left ? __ffs(left) - 1 : l0;
-      const bool two = left != 0;
-      left &= left - 1;
-      const int l = lane < 16 ? l0 : l1, t0 = __shfl_sync(0xffffffffu, at, l);
-      look(Tile<T>::token(t0 * TILE, l, lane & 15), lane < 16 || two);
+    const auto look = [&]() {
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q)
+        if (__any_sync(0xffffffffu, f[q] >= least)) offer(best, wv, wi, f[q], f[q] >= least ? token[q] : RowBest::NONE, W, lane);
+    };
+    for (uint32_t left = lanes & ~whole; left;) {      // one tile of each lane's tokens, two lanes at a time
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) {
+        const int l0 = __ffs(left) - 1;
+        const bool one = left != 0;
+        left &= left - 1;
+        const int l1 = __ffs(left) - 1;
+        const bool two = left != 0;
+        left &= left - 1;
+        const int l = max(0, lane < 16 ? l0 : l1), t0 = __shfl_sync(0xffffffffu, at, l);
+        ask(q, Tile<T>::token(t0 * TILE, l, lane & 15), lane < 16 ? one : two);
+      }
+      look();
     }
     for (uint32_t left = whole; left; left &= left - 1) {      // all tiles of a lane's
       const int l = __ffs(left) - 1, n = (hi - lo) * 16;
-      for (int e = lane; e - lane < n; e += 32) look(Tile<T>::token((lo + (e >> 4)) * TILE, l, e & 15), e < n);
+      for (int e = lane; e - lane < n; e += 32 * AHEAD) {
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) ask(q, Tile<T>::token((lo + ((e + 32 * q) >> 4)) * TILE, l, e & 15), e + 32 * q < n);
+        look();
+      }
     }
   }
   // the warp's sum, relative to its maximum
