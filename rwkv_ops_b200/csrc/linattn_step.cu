@@ -69,8 +69,7 @@ __global__ void __launch_bounds__(STEP_THR) la_step_kernel(const T* __restrict__
   for (int j = 0; j < W; ++j) {
     if (j < beams) {
       const long long seq = (long long)g * beams + j, at = (seq * H + h) * D;
-      // (exact in the decay: what a step loses here, it loses every token)
-      const float d = (float)exp(g_of(__ldg(w + seq * w_stride + h)));
+      const float d = decay_of(__ldg(w + seq * w_stride + h));      // (in float64 this was half the time of a step with beams)
       float rr[KQ], kk[KQ];
 #pragma unroll
       for (int c = 0; c < KQ; c += 4) {
