@@ -145,23 +145,43 @@ struct Cut {
   bool chained() const { return adds() > 12; }      // put together by a kernel of its own; otherwise by each part, at its start
 };
 struct Stretch { int unit, part, n, h, len, NT, lo, hi; };
-__device__ __forceinline__ Stretch unit_of(const Tokens& t, const Cut& cut) {
+// PACKED: the units in the order of their lengths, the longest first, where a thread can compare one sequence with all others; a unit that starts last
+// then is a short one.  All threads call it; `slot` is shared memory.
+template <bool PACKED>
+__device__ __forceinline__ Stretch unit_of(const Tokens& t, const Cut& cut, int* slot) {
   Stretch x;
   x.unit = blockIdx.x % cut.n_units; x.part = blockIdx.x / cut.n_units;
   x.n = x.unit / t.H; x.h = x.unit % t.H;
+  if (PACKED && t.n_seq <= (int)blockDim.x) {
+    const int me = threadIdx.x;
+    if (me < t.n_seq) {
+      const int len = __ldg(t.len + me);
+      int place = 0;
+      for (int q = 0; q < t.n_seq; ++q) {
+        const int other = __ldg(t.len + q);
+        place += other > len || (other == len && q < me);
+      }
+      if (place == x.n) *slot = me;
+    }
+    __syncthreads();
+    x.n = *slot;
+    x.unit = x.n * t.H + x.h;
+  }
   x.len = t.length(x.n);
   x.NT = (x.len + CT - 1) / CT;
   return x;
 }
-__device__ __forceinline__ Stretch stretch_of(const Tokens& t, const Cut& cut) {
-  Stretch x = unit_of(t, cut);
+template <bool PACKED>
+__device__ __forceinline__ Stretch stretch_of(const Tokens& t, const Cut& cut, int* slot) {
+  Stretch x = unit_of<PACKED>(t, cut, slot);
   x.lo = min(x.part * cut.per, x.NT);
   x.hi = min(x.lo + cut.per, x.NT);
   return x;
 }
 // a piece of the pass that adds: `part` counts the pieces of a unit, in the order of the chunks
-__device__ __forceinline__ Stretch piece_of(const Tokens& t, const Cut& cut, bool reverse) {
-  Stretch x = unit_of(t, cut);
+template <bool PACKED>
+__device__ __forceinline__ Stretch piece_of(const Tokens& t, const Cut& cut, bool reverse, int* slot) {
+  Stretch x = unit_of<PACKED>(t, cut, slot);
   const int p = x.part / cut.sub + reverse, s = x.part % cut.sub;
   x.lo = min(p * cut.per + s * cut.per_sub, x.NT);
   x.hi = min(min(x.lo + cut.per_sub, (p + 1) * cut.per), x.NT);

@@ -25,6 +25,7 @@ struct BwdSmem {
   uint64_t bar_ae, bar_read;                 // of all warps: A and E are stored; r and k have been read
   uint64_t bar_free, bar_r;                  // the staged gradients have left; the scaled r is stored
   uint32_t tmem_base;
+  int sequence;
 };
 // The warps whose block of pairs lies above the diagonal (4, 8, 9, 12, 13, 14) do the other jobs: ISSUE the products (a thread that issues is held up by those
 // under way, some 50 cycles each), STORE the copies of the gradients, DECAYS the next chunk's decays, DW the dw of the chunk before and (LOAD) the loads, and
@@ -95,7 +96,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
   earlier_kernels_done();
   later_kernels_may_start();
   const uint32_t tm = sm.tmem_base;
-  const Stretch x = stretch_of(tok, cut);
+  const Stretch x = stretch_of<PACKED>(tok, cut, &sm.sequence);
   const int seq0 = PACKED ? __ldg(tok.start + x.n) : 0, brow = PACKED ? 0 : x.n;
   const long long wb = tok.wbase(x.n, x.h), at = tok.base(x.n, x.h) + (long long)row * tok.st + 16 * qt;      // of w; of this thread's part of a row
   auto rows_of = [&](int c) { return min(CT, x.len - c * CT); };

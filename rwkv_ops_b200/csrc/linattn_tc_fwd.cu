@@ -20,12 +20,14 @@ struct FwdSmem {
   Decays dec[2];
   uint64_t bar_in, bar_1, bar_2;
   uint32_t tmem_base;
+  int sequence;
 };
 struct AddSmem {      // keys and values alone: three CTAs to an SM
   unsigned char k[TOK_BYTES], v[TOK_BYTES], klo[TOK_BYTES];
   Decays dec[2];
   uint64_t bar_in, bar_1, bar_2;
   uint32_t tmem_base;
+  int sequence;
 };
 constexpr uint32_t TM_S = 0, TM_O2 = 0, TM_O1 = 128;
 
@@ -60,7 +62,7 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
   earlier_kernels_done();
   later_kernels_may_start();
   const uint32_t tm = sm.tmem_base;
-  const Stretch x = ADD ? piece_of(tok, cut, REV) : stretch_of(tok, cut);
+  const Stretch x = ADD ? piece_of<PACKED>(tok, cut, REV, &sm.sequence) : stretch_of<PACKED>(tok, cut, &sm.sequence);
   const int seq0 = PACKED ? __ldg(tok.start + x.n) : 0, brow = PACKED ? 0 : x.n;
   const long long wb = tok.wbase(x.n, x.h), at = tok.base(x.n, x.h) + (long long)row * tok.st + 32 * half;      // of w; of this thread's part of a row
   auto rows_of = [&](int c) { return min(CT, x.len - c * CT); };
