@@ -15,15 +15,15 @@ constexpr int PAD = 4;        // rows of shared tiles are 4 floats longer: 16-by
 constexpr int LD = 64 + PAD;
 constexpr int NTHR = 256;
 
-// acc[a][b] += sum over kk < n of A(ig + 16 a, kk) B(kk, jg + 16 b).  AM / BM: the contraction index is the row of the array
+// acc[a][b] += sum over kk < n of A(ig + 16 a, kk) B(kk, jg + 16 b), RA rows a.  AM / BM: the contraction index is the row of the array
 // (A[kk][i], B[kk][j]) instead of its column (A[i][kk], B[j][kk]).
-template <bool AM, bool BM>
-__device__ __forceinline__ void mm(float (&acc)[4][4], const float* A, int lda, const float* B, int ldb, int n, int ig, int jg) {
+template <bool AM, bool BM, int RA>
+__device__ __forceinline__ void mm(float (&acc)[RA][4], const float* A, int lda, const float* B, int ldb, int n, int ig, int jg) {
 #pragma unroll 4
   for (int kk = 0; kk < n; kk += 4) {
-    float a[4][4], b[4][4];
+    float a[RA][4], b[4][4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    for (int x = 0; x < RA; ++x) {
       if constexpr (AM) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) a[x][c] = A[(kk + c) * lda + ig + 16 * x];
@@ -31,6 +31,9 @@ __device__ __forceinline__ void mm(float (&acc)[4][4], const float* A, int lda, 
         const float4 f = *reinterpret_cast<const float4*>(A + (ig + 16 * x) * lda + kk);
         a[x][0] = f.x; a[x][1] = f.y; a[x][2] = f.z; a[x][3] = f.w;
       }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
       if constexpr (BM) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) b[x][c] = B[(kk + c) * ldb + jg + 16 * x];
@@ -42,14 +45,15 @@ __device__ __forceinline__ void mm(float (&acc)[4][4], const float* A, int lda, 
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+      for (int x = 0; x < RA; ++x)
 #pragma unroll
         for (int y = 0; y < 4; ++y) acc[x][y] = fmaf(a[x][c], b[y][c], acc[x][y]);
   }
 }
-__device__ __forceinline__ void clear(float (&acc)[4][4]) {
+template <int RA>
+__device__ __forceinline__ void clear(float (&acc)[RA][4]) {
 #pragma unroll
-  for (int x = 0; x < 4; ++x)
+  for (int x = 0; x < RA; ++x)
 #pragma unroll
     for (int y = 0; y < 4; ++y) acc[x][y] = 0.f;
 }
@@ -57,7 +61,7 @@ __device__ __forceinline__ void clear(float (&acc)[4][4]) {
 // Rows 0 .. 63 (the first n of them from p with `stride` elements between rows, zeros behind) of W columns, as float32.
 template <typename T, int W>
 __device__ __forceinline__ void load_rows(float* dst, int ld, const T* p, long long stride, int n) {
-  for (int i = threadIdx.x; i < 64 * (W / 4); i += NTHR) {
+  for (int i = threadIdx.x; i < 64 * (W / 4); i += blockDim.x) {
     const int row = i / (W / 4), c = i % (W / 4) * 4;
     const float4 f = row < n ? load4(p + row * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
     *reinterpret_cast<float4*>(dst + row * ld + c) = f;
@@ -136,8 +140,7 @@ __global__ void __launch_bounds__(256) la_scan_kernel(float* __restrict__ states
   earlier_kernels_done();
   later_kernels_may_start();
   constexpr int PER = D * D / 4;
-  const int i = blockIdx.x * 256 + threadIdx.x, unit = i / PER, e = 4 * (i % PER);
-  if (unit >= tok.n_seq * tok.H) return;
+  const int unit = blockIdx.x / (PER / 256), e = 4 * ((blockIdx.x % (PER / 256)) * 256 + threadIdx.x);
   const int n = unit / tok.H, h = unit % tok.H, NT = (tok.length(n) + C - 1) / C;
   float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
   if (first && n_first > 0) S = *reinterpret_cast<const float4*>(first + ((long long)(n_first == 1 ? 0 : n) * tok.H + h) * (D * D) + e);
@@ -223,10 +226,11 @@ __global__ void __launch_bounds__(NTHR) la_out_kernel(const T* __restrict__ r, c
   }
 }
 
+constexpr int G_THR = 2 * NTHR;      // of the gradient kernel
 template <int D> struct GradSmem {
-  float r[64 * (D + PAD)], k[64 * (D + PAD)], v[64 * (D + PAD)], d_o[64 * (D + PAD)], A[64 * LD], E[64 * LD], S[64 * LD];
+  float r[64 * (D + PAD)], k[64 * (D + PAD)], v[64 * (D + PAD)], d_o[64 * (D + PAD)], A[64 * LD], E[64 * LD], S[2][64 * LD];
   double L[C], g[C];
-  float pairs[NTHR / 32][C], t1[C], t2[C], t3[NTHR / 32];
+  float pairs[G_THR / 32][C], t1[C], t2[C], t3[G_THR / 32];
 };
 // The sum of x over the 16 threads that hold a row's columns.
 __device__ __forceinline__ float row_sum(float x) {
@@ -235,16 +239,17 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
-// The gradients of a chunk.  dstates: slot c + 1 is the gradient of the state after chunk c.
+// The gradients of a chunk.  dstates: slot c + 1 is the gradient of the state after chunk c.  Two halves of the block work on a product each: one on r k^T and
+// dr, the other on d_o v^T and dk, and on dv half its rows each (16 warps to an SM instead of 8: B2 T1024 H16 float32 121 -> 80 us).
 template <typename T, int D>
-__global__ void __launch_bounds__(NTHR) la_grad_kernel(const T* __restrict__ r, const T* __restrict__ k, const T* __restrict__ v,
-                                                       const float* __restrict__ w, const T* __restrict__ d_o,
-                                                       const float* __restrict__ states, const float* __restrict__ dstates,
-                                                       T* __restrict__ dr, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ dw,
-                                                       int dw_rows, Tokens tok) {
+__global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r, const T* __restrict__ k, const T* __restrict__ v,
+                                                        const float* __restrict__ w, const T* __restrict__ d_o,
+                                                        const float* __restrict__ states, const float* __restrict__ dstates,
+                                                        T* __restrict__ dr, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ dw,
+                                                        int dw_rows, Tokens tok) {
   extern __shared__ __align__(16) unsigned char raw[];
   GradSmem<D>& sm = *reinterpret_cast<GradSmem<D>*>(raw);
-  constexpr int LDD = D + PAD, P = D / 64;
+  constexpr int LDD = D + PAD, P = D / 64, NW = G_THR / 32;
   earlier_kernels_done();
   later_kernels_may_start();
   const int c = blockIdx.x % tok.NT, unit = blockIdx.x / tok.NT, tid = threadIdx.x;
@@ -258,11 +263,12 @@ __global__ void __launch_bounds__(NTHR) la_grad_kernel(const T* __restrict__ r, 
   load_rows<T, D>(sm.d_o, LDD, d_o + base, tok.st, x.rows);
   const float* S0 = states + ((long long)unit * (tok.NT + 1) + c) * (D * D);
   const float* dS = dstates + ((long long)unit * (tok.NT + 1) + c + 1) * (D * D);
-  const int ig = tid >> 4, jg = tid & 15, warp = tid >> 5, lane = tid & 31;
+  const bool first = tid < NTHR;      // which half
+  const int ig = (tid & (NTHR - 1)) >> 4, jg = tid & 15, warp = tid >> 5, lane = tid & 31;
   // <dS, S0>
   {
     float s = 0.f;
-    for (int i = 4 * tid; i < D * D; i += 4 * NTHR) {
+    for (int i = 4 * tid; i < D * D; i += 4 * G_THR) {
       const float4 a = load4(S0 + i), b = load4(dS + i);
       s += a.x * b.x + a.y * b.y + a.z * b.z + a.w * b.w;
     }
@@ -271,31 +277,36 @@ __global__ void __launch_bounds__(NTHR) la_grad_kernel(const T* __restrict__ r, 
     if (lane == 0) sm.t3[warp] = s;
   }
   __syncthreads();
-  float acc[4][4], pr[4][4];
+  float acc[4][4];
   clear(acc);
-  mm<false, false>(acc, sm.r, LDD, sm.k, LDD, D, ig, jg);
-  clear(pr);
-  mm<false, false>(pr, sm.d_o, LDD, sm.v, LDD, D, ig, jg);
+  mm<false, false>(acc, first ? sm.r : sm.d_o, LDD, first ? sm.k : sm.v, LDD, D, ig, jg);
 #pragma unroll
   for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
       const int i = ig + 16 * a, j = jg + 16 * b;
-      const float f = j <= i ? expf((float)(sm.L[i] - sm.L[j])) : 0.f;
-      const float A = j <= i ? acc[a][b] * f : 0.f;      // (a choice, so that infinities above the diagonal stay there)
-      sm.A[i * LD + j] = A;
-      sm.E[i * LD + j] = j <= i ? pr[a][b] * f : 0.f;
-      sm.S[i * LD + j] = j < i ? A * pr[a][b] : 0.f;     // (the diagonal does not depend on the decay)
+      (first ? sm.A : sm.E)[i * LD + j] = j <= i ? acc[a][b] * expf((float)(sm.L[i] - sm.L[j])) : 0.f;      // (a choice, so that infinities above the diagonal stay there)
     }
+  __syncthreads();
+  if (!first) {
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const int i = ig + 16 * a, j = jg + 16 * b;
+        sm.S[0][i * LD + j] = j < i ? sm.A[i * LD + j] * acc[a][b] : 0.f;      // (the diagonal does not depend on the decay)
+      }
+  }
+  if (tid < C) { sm.t1[tid] = 0.f; sm.t2[tid] = 0.f; }
   __syncthreads();
   {
     // What the pairs on both sides of t add to dg_t: prefix sums along the rows, then their columns from the diagonal down.  Every term of such a
     // sum carries the decay of t, so a token whose decay is strong gets a gradient that is as exact as any.
-    float x[2] = {0.f, 0.f};
+    float y[2] = {0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < 64 / (NTHR / 32); ++q) {
-      const int i = warp + (NTHR / 32) * q;
-      const float2 m = *reinterpret_cast<const float2*>(&sm.S[i * LD + 2 * lane]);
+    for (int q = 0; q < 64 / NW; ++q) {
+      const int i = warp + NW * q;
+      const float2 m = *reinterpret_cast<const float2*>(&sm.S[0][i * LD + 2 * lane]);
       float s = m.x + m.y;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
@@ -304,20 +315,43 @@ __global__ void __launch_bounds__(NTHR) la_grad_kernel(const T* __restrict__ r, 
       }
       const float left = __shfl_up_sync(0xffffffffu, s, 1);
       const float p0 = lane ? left : 0.f;      // sum of the columns before 2 lane
-      if (2 * lane <= i) x[0] += p0;
-      if (2 * lane + 1 <= i) x[1] += p0 + m.x;
+      if (2 * lane <= i) y[0] += p0;
+      if (2 * lane + 1 <= i) y[1] += p0 + m.x;
     }
-    sm.pairs[warp][2 * lane] = x[0];
-    sm.pairs[warp][2 * lane + 1] = x[1];
+    sm.pairs[warp][2 * lane] = y[0];
+    sm.pairs[warp][2 * lane + 1] = y[1];
   }
-  if (tid < C) { sm.t1[tid] = 0.f; sm.t2[tid] = 0.f; }
-  float eL[4], eR[4];
+  float f[4];      // the decay between a row's token and the state: before the chunk, behind it
 #pragma unroll
-  for (int a = 0; a < 4; ++a) {
-    eL[a] = expf((float)sm.L[ig + 16 * a]);
-    eR[a] = expf((float)(sm.L[C - 1] - sm.L[ig + 16 * a]));
-  }
-  auto store = [&](T* out, int p) {
+  for (int a = 0; a < 4; ++a) f[a] = expf((float)(first ? sm.L[ig + 16 * a] : sm.L[C - 1] - sm.L[ig + 16 * a]));
+  const int row0 = first ? 0 : 32;      // of dv
+  float fv[2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a) fv[a] = expf((float)(sm.L[C - 1] - sm.L[row0 + ig + 16 * a]));
+  for (int p = 0; p < P; ++p) {      // 64 columns of each gradient
+    clear(acc);
+    for (int pv = 0; pv < P; ++pv) {
+      __syncthreads();
+      load_rows<float, 64>(sm.S[0], LD, S0 + 64 * pv * D + 64 * p, D, 64);
+      load_rows<float, 64>(sm.S[1], LD, dS + 64 * pv * D + 64 * p, D, 64);
+      __syncthreads();
+      mm<false, true>(acc, (first ? sm.d_o : sm.v) + 64 * pv, LDD, sm.S[first ? 0 : 1], LD, 64, ig, jg);
+    }
+    const float* q = (first ? sm.r : sm.k) + 64 * p;      // (what it is multiplied with in dg)
+#pragma unroll
+    for (int a = 0; a < 4; ++a) {
+      float s = 0.f;
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        acc[a][b] *= f[a];
+        s += acc[a][b] * q[(ig + 16 * a) * LDD + jg + 16 * b];
+      }
+      s = row_sum(s);
+      if (jg == 0) (first ? sm.t1 : sm.t2)[ig + 16 * a] += s;
+    }
+    if (first) mm<false, true>(acc, sm.E, LD, sm.k + 64 * p, LDD, 64, ig, jg);
+    else       mm<true, true>(acc, sm.E, LD, sm.r + 64 * p, LDD, 64, ig, jg);
+    T* out = first ? dr : dk;
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
       const int i = ig + 16 * a;
@@ -326,53 +360,29 @@ __global__ void __launch_bounds__(NTHR) la_grad_kernel(const T* __restrict__ r, 
         for (int b = 0; b < 4; ++b) out[base + i * tok.st + 64 * p + jg + 16 * b] = from_f32<T>(acc[a][b]);
       }
     }
-  };
-  auto load_S = [&](const float* from, int pv, int pk) {      // (everyone has read the one before, and will see this one)
-    __syncthreads();
-    load_rows<float, 64>(sm.S, LD, from + 64 * pv * D + 64 * pk, D, 64);
-    __syncthreads();
-  };
-  // scale the state's part by f, add its products with the rows of q to the sums t
-  auto state_part = [&](const float (&f)[4], const float* q, float* t) {
-#pragma unroll
-    for (int a = 0; a < 4; ++a) {
-      float s = 0.f;
-#pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        acc[a][b] *= f[a];
-        if (q) s += acc[a][b] * q[(ig + 16 * a) * LDD + jg + 16 * b];
-      }
-      if (q) {
-        s = row_sum(s);
-        if (jg == 0) t[ig + 16 * a] += s;
-      }
-    }
-  };
-  for (int p = 0; p < P; ++p) {      // 64 columns of each gradient
-    clear(acc);
-    for (int pv = 0; pv < P; ++pv) {
-      load_S(S0, pv, p);
-      mm<false, true>(acc, sm.d_o + 64 * pv, LDD, sm.S, LD, 64, ig, jg);
-    }
-    state_part(eL, sm.r + 64 * p, sm.t1);
-    mm<false, true>(acc, sm.E, LD, sm.k + 64 * p, LDD, 64, ig, jg);
-    store(dr, p);
-    clear(acc);
-    for (int pv = 0; pv < P; ++pv) {
-      load_S(dS, pv, p);
-      mm<false, true>(acc, sm.v + 64 * pv, LDD, sm.S, LD, 64, ig, jg);
-    }
-    state_part(eR, sm.k + 64 * p, sm.t2);
-    mm<true, true>(acc, sm.E, LD, sm.r + 64 * p, LDD, 64, ig, jg);
-    store(dk, p);
-    clear(acc);
+    float av[2][4];
+    clear(av);
     for (int pk = 0; pk < P; ++pk) {
-      load_S(dS, p, pk);
-      mm<false, false>(acc, sm.k + 64 * pk, LDD, sm.S, LD, 64, ig, jg);
+      if (P > 1) {      // (otherwise it is there)
+        __syncthreads();
+        load_rows<float, 64>(sm.S[1], LD, dS + 64 * p * D + 64 * pk, D, 64);
+        __syncthreads();
+      }
+      mm<false, false>(av, sm.k + row0 * LDD + 64 * pk, LDD, sm.S[1], LD, 64, ig, jg);
     }
-    state_part(eR, nullptr, nullptr);
-    mm<true, true>(acc, sm.A, LD, sm.d_o + 64 * p, LDD, 64, ig, jg);
-    store(dv, p);
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int b = 0; b < 4; ++b) av[a][b] *= fv[a];
+    mm<true, true>(av, sm.A + row0, LD, sm.d_o + 64 * p, LDD, 64, ig, jg);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      const int i = row0 + ig + 16 * a;
+      if (i < x.rows) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) dv[base + i * tok.st + 64 * p + jg + 16 * b] = from_f32<T>(av[a][b]);
+      }
+    }
   }
   __syncthreads();
   if (warp == 0) {      // dg_t, two tokens to a lane
@@ -382,7 +392,7 @@ __global__ void __launch_bounds__(NTHR) la_grad_kernel(const T* __restrict__ r, 
       const int i = 2 * lane + q;
       pairs[q] = 0.0;
 #pragma unroll
-      for (int u = 0; u < NTHR / 32; ++u) pairs[q] += sm.pairs[u][i];
+      for (int u = 0; u < NW; ++u) pairs[q] += sm.pairs[u][i];
       after[q] = sm.t1[i];
       before[q] = sm.t2[i];
     }
@@ -395,7 +405,7 @@ __global__ void __launch_bounds__(NTHR) la_grad_kernel(const T* __restrict__ r, 
     }
     double t3 = 0.0;
 #pragma unroll
-    for (int u = 0; u < NTHR / 32; ++u) t3 += sm.t3[u];
+    for (int u = 0; u < NW; ++u) t3 += sm.t3[u];
     t3 *= exp(sm.L[C - 1]);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
@@ -502,7 +512,7 @@ int bwd(const Args& a, cudaStream_t st) {
     ProfScope prof("linattn_grad_kernel", st);
     constexpr int smem = (int)sizeof(GradSmem<D>);
     if (int e = allow_smem<la_grad_kernel<T, D>>(f, smem)) return e;
-    if (int e = launch(la_grad_kernel<T, D>, t.NT * units, NTHR, smem, st, 1, (const T*)a.r, (const T*)a.k, (const T*)a.v, a.w, (const T*)a.d_o,
+    if (int e = launch(la_grad_kernel<T, D>, t.NT * units, G_THR, smem, st, 1, (const T*)a.r, (const T*)a.k, (const T*)a.v, a.w, (const T*)a.d_o,
                        (const float*)a.states, (const float*)s.dstates, (T*)a.dr, (T*)a.dk, (T*)a.dv, a.w_per_head ? s.dw : a.dw, a.w_per_head, t)) return e;
   }
   return a.w_per_head ? launch_sum_dw(s.dw, a.w_rows, t.H, s.part, a.dw, st) : RWKVB200_OK;

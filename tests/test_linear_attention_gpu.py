@@ -115,6 +115,65 @@ def test_packed(dtype, D, w, n_state):
     assert torch.isnan(other["o"][:, 131:195]).all()
 
 
+@pytest.mark.parametrize("B,T,H,w,with_state", [
+    (1, 2100, 1, "token", True),       # every chunk of 128 a part of its own, chained by a kernel
+    (1, 1500, 1, "head", True),        # parts that put their start together themselves
+    (9, 3000, 11, "token", False),     # two parts forward, the pass before them in finer pieces; one part backward
+    (1, 5000, 24, "head", True),       # parts in both directions, the last chunk cut short
+    (2, 1100, 37, "token", True),
+])
+def test_parts_of_few_sequences_are_the_whole(B, T, H, w, with_state):
+    """Few sequences are walked in parts at once; bfloat16 tokens against the float32 operator, which has no parts, on the same values."""
+    import rwkv_ops_b200 as ro
+    g = torch.Generator(device="cuda").manual_seed(T)
+
+    def n(*s):
+        return torch.randn(*s, generator=g, device="cuda")
+
+    x = [n(B, T, H, 64).bfloat16(), (-3 + n(H) if w == "head" else -3 + n(B, T, H)), (n(B, T, H, 64) / 8).bfloat16(), n(B, T, H, 64).bfloat16()]
+    s0 = 0.1 * n(B, H, 64, 64) if with_state else None
+    d_o, d_s = n(B, T, H, 64).bfloat16(), 0.1 * n(B, H, 64, 64)
+
+    def call(dtype):
+        a = [t if t.dtype == F32 else t.to(dtype) for t in x]
+        a = [t.requires_grad_(True) for t in (u.detach().clone() for u in a)]
+        s = None if s0 is None else s0.clone().requires_grad_(True)
+        o, ht = ro.linear_attention(*a, initial_state=s)
+        wrt = a if s is None else a + [s]
+        return dict(zip(["o", "s", "dr", "dw", "dk", "dv", "ds0"], [o, ht, *torch.autograd.grad((o, ht), wrt, (d_o.to(dtype), d_s))]))
+
+    ref.check(call(BF16), {q: t.detach().double().cpu() for q, t in call(F32).items()}, BF16)
+
+
+def test_parts_of_packed_sequences():
+    """Packed sequences of very different lengths, few enough to be walked in parts: short ones have none of the later parts."""
+    import rwkv_ops_b200 as ro
+    lens, H = [2500, 3, 700, 128, 1], 3
+    cu = torch.tensor([0] + lens).cumsum(0)
+    T = int(cu[-1])
+    g = torch.Generator(device="cuda").manual_seed(22)
+
+    def n(*s):
+        return torch.randn(*s, generator=g, device="cuda")
+
+    x = [n(1, T, H, 64).bfloat16(), -3 + n(1, T, H), (n(1, T, H, 64) / 8).bfloat16(), n(1, T, H, 64).bfloat16()]
+    s0, d_o, d_s = 0.1 * n(5, H, 64, 64), n(1, T, H, 64).bfloat16(), 0.1 * n(5, H, 64, 64)
+    x = [t.requires_grad_(True) for t in x]
+    s0.requires_grad_(True)
+    o, s = ro.linear_attention_varlen(*x, cu, initial_state=s0)
+    packed = dict(zip(["o", "s", "dr", "dw", "dk", "dv", "ds0"], [o, s, *torch.autograd.grad((o, s), [*x, s0], (d_o, d_s))]))
+    alone = []
+    for i in range(5):
+        cut = slice(int(cu[i]), int(cu[i + 1]))
+        y = [t[:, cut].detach().to(BF16 if t.dim() == 4 else F32).float().requires_grad_(True) for t in x]
+        z = s0[i:i + 1].detach().requires_grad_(True)
+        o, s = ro.linear_attention(*y, initial_state=z)
+        alone.append([o, s, *torch.autograd.grad((o, s), [*y, z], (d_o[:, cut].float(), d_s[i:i + 1]))])
+    want = {q: torch.cat([a[j] for a in alone], 0 if q in ("s", "ds0") else 1).detach().double().cpu()
+            for j, q in enumerate(["o", "s", "dr", "dw", "dk", "dv", "ds0"])}
+    ref.check(packed, want, BF16)
+
+
 def test_gradients_are_differences():
     """A directional derivative of a scalar of the outputs, against central differences of the float64 definition and of the operator itself."""
     import rwkv_ops_b200 as ro
