@@ -28,8 +28,9 @@
 namespace rwkvb200 {
 namespace la {
 
-constexpr double G_FLOOR = -200.0;
-__device__ __forceinline__ double g_of(float w) { return fmax(-exp((double)w), G_FLOOR); }
+// g is a float32 exponential and only its sums are float64: an error of 2^-23 of L, times e^L, is never more than 2^-24.
+constexpr float G_FLOOR = -200.f;
+__device__ __forceinline__ float g_of(float w) { return fmaxf(-expf(w), G_FLOOR); }
 
 // Where the tokens lie.  Token tensors have strides sb / st / sh (elements) over batch, token and head, w its own (zero over
 // batch and token where it is a number per head).  Dense: sequence n is batch row n with T tokens; packed (start != nullptr): all

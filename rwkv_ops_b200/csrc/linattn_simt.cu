@@ -15,28 +15,32 @@ constexpr int PAD = 4;        // rows of shared tiles are 4 floats longer: 16-by
 constexpr int LD = 64 + PAD;
 constexpr int NTHR = 256;
 
-// acc[a][b] += sum over kk < n of A(ig + 16 a, kk) B(kk, jg + 16 b), RA rows a.  AM / BM: the contraction index is the row of the array
-// (A[kk][i], B[kk][j]) instead of its column (A[i][kk], B[j][kk]).
+// acc[a][b] += sum over kk < n of A(RA ig + a, kk) B(kk, j).  AM / BM: the contraction index is the row of the array (A[kk][i], B[kk][j]) instead of its
+// column (A[i][kk], B[j][kk]).  Columns j: 4 jg + b with BM, so that they are one read, else jg + 16 b, so that 16 rows' reads do not conflict.  A warp's
+// two ig and 16 jg take 12 shared-memory cycles for 64 multiply-adds in every form, below the 16 that these take.
 template <bool AM, bool BM, int RA>
 __device__ __forceinline__ void mm(float (&acc)[RA][4], const float* A, int lda, const float* B, int ldb, int n, int ig, int jg) {
 #pragma unroll 4
   for (int kk = 0; kk < n; kk += 4) {
     float a[RA][4], b[4][4];
 #pragma unroll
-    for (int x = 0; x < RA; ++x) {
-      if constexpr (AM) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) a[x][c] = A[(kk + c) * lda + ig + 16 * x];
-      } else {
-        const float4 f = *reinterpret_cast<const float4*>(A + (ig + 16 * x) * lda + kk);
+    for (int x = 0; x < (AM ? 4 : RA); ++x) {
+      if constexpr (!AM) {
+        const float4 f = *reinterpret_cast<const float4*>(A + (RA * ig + x) * lda + kk);
         a[x][0] = f.x; a[x][1] = f.y; a[x][2] = f.z; a[x][3] = f.w;
+      } else if constexpr (RA == 4) {
+        const float4 f = *reinterpret_cast<const float4*>(A + (kk + x) * lda + 4 * ig);
+        a[0][x] = f.x; a[1][x] = f.y; a[2][x] = f.z; a[3][x] = f.w;
+      } else {
+        const float2 f = *reinterpret_cast<const float2*>(A + (kk + x) * lda + 2 * ig);
+        a[0][x] = f.x; a[1][x] = f.y;
       }
     }
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       if constexpr (BM) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) b[x][c] = B[(kk + c) * ldb + jg + 16 * x];
+        const float4 f = *reinterpret_cast<const float4*>(B + (kk + x) * ldb + 4 * jg);
+        b[0][x] = f.x; b[1][x] = f.y; b[2][x] = f.z; b[3][x] = f.w;
       } else {
         const float4 f = *reinterpret_cast<const float4*>(B + (jg + 16 * x) * ldb + kk);
         b[x][0] = f.x; b[x][1] = f.y; b[x][2] = f.z; b[x][3] = f.w;
@@ -68,20 +72,34 @@ __device__ __forceinline__ void load_rows(float* dst, int ld, const T* p, long l
   }
 }
 
-// Inclusive prefix sums of g over a chunk of n tokens, by the first warp; L[63] is the sum over the chunk.
-__device__ __forceinline__ void prefix(double* L, double* g, const Tokens& t, const float* w, long long wb, int t0, int n) {
+// 64 rows of 64 columns of a state, transposed.
+__device__ __forceinline__ void load_transposed(float* dst, const float* p, int stride) {
+  for (int i = threadIdx.x; i < 64 * 16; i += blockDim.x) {
+    const int row = i & 63, c = i >> 6 << 2;      // (a warp's 32 rows: writes next to each other)
+    const float4 f = load4(p + row * stride + c);
+    dst[c * LD + row] = f.x; dst[(c + 1) * LD + row] = f.y; dst[(c + 2) * LD + row] = f.z; dst[(c + 3) * LD + row] = f.w;
+  }
+}
+
+// Inclusive prefix sums of g over a chunk, each as two floats: sums and differences of them are exact to far below float32's last bit, and the many
+// differences that are taken cost no float64 arithmetic (of which an SM does little: with it the gradient kernel took a third longer).
+struct Sums { float hi[C], lo[C]; };
+__device__ __forceinline__ float between(const Sums& L, int i, int j) { return (L.hi[i] - L.hi[j]) + (L.lo[i] - L.lo[j]); }
+// by the first warp, of n tokens (those behind do not decay); L[63] is the sum over the chunk
+__device__ __forceinline__ void prefix(Sums& L, float* g, const Tokens& t, const float* w, long long wb, int t0, int n) {
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x, i = 2 * lane;
-    const double g0 = i < n ? g_of(w[wb + (t0 + i) * t.wst]) : 0.0;
-    const double g1 = i + 1 < n ? g_of(w[wb + (t0 + i + 1) * t.wst]) : 0.0;
-    double s = g0 + g1;
+    const float g0 = i < n ? g_of(w[wb + (t0 + i) * t.wst]) : 0.f;
+    const float g1 = i + 1 < n ? g_of(w[wb + (t0 + i + 1) * t.wst]) : 0.f;
+    double s = (double)g0 + (double)g1;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const double up = __shfl_up_sync(0xffffffffu, s, d);
       if (lane >= d) s += up;
     }
-    L[i] = s - g1;
-    L[i + 1] = s;
+    const double s0 = s - (double)g1;
+    L.hi[i] = (float)s0; L.lo[i] = (float)(s0 - (double)L.hi[i]);
+    L.hi[i + 1] = (float)s; L.lo[i + 1] = (float)(s - (double)L.hi[i + 1]);
     if (g) { g[i] = g0; g[i + 1] = g1; }
   }
 }
@@ -103,7 +121,7 @@ template <typename T, int D, bool REV>
 __global__ void __launch_bounds__(NTHR) la_add_kernel(const T* __restrict__ val, const T* __restrict__ key, const float* __restrict__ w,
                                                       float* __restrict__ states, float* __restrict__ decay, Tokens tok) {
   __shared__ __align__(16) float av[64 * LD], bk[64 * LD];
-  __shared__ double L[C];
+  __shared__ Sums L;
   earlier_kernels_done();
   later_kernels_may_start();
   const int c = blockIdx.x % tok.NT, unit = blockIdx.x / tok.NT, pv = blockIdx.y / (D / 64), pk = blockIdx.y % (D / 64);
@@ -116,7 +134,7 @@ __global__ void __launch_bounds__(NTHR) la_add_kernel(const T* __restrict__ val,
   __syncthreads();
   for (int i = threadIdx.x; i < 64 * 64; i += NTHR) {
     const int j = i >> 6;
-    bk[j * LD + (i & 63)] *= expf((float)(REV ? L[j] : L[C - 1] - L[j]));
+    bk[j * LD + (i & 63)] *= expf(REV ? L.hi[j] : between(L, C - 1, j));
   }
   __syncthreads();
   const int ig = threadIdx.x >> 4, jg = threadIdx.x & 15;
@@ -125,10 +143,8 @@ __global__ void __launch_bounds__(NTHR) la_add_kernel(const T* __restrict__ val,
   mm<true, true>(acc, av, LD, bk, LD, 64, ig, jg);
   float* out = states + ((long long)unit * (tok.NT + 1) + (REV ? c : c + 1)) * (D * D) + (64 * pv) * D + 64 * pk;
 #pragma unroll
-  for (int a = 0; a < 4; ++a)
-#pragma unroll
-    for (int b = 0; b < 4; ++b) out[(ig + 16 * a) * D + jg + 16 * b] = acc[a][b];
-  if (blockIdx.y == 0 && threadIdx.x == 0) decay[(long long)unit * tok.NT + c] = expf((float)L[C - 1]);
+  for (int a = 0; a < 4; ++a) store4(out + (4 * ig + a) * D + 4 * jg, make_float4(acc[a][0], acc[a][1], acc[a][2], acc[a][3]));
+  if (blockIdx.y == 0 && threadIdx.x == 0) decay[(long long)unit * tok.NT + c] = expf(L.hi[C - 1]);
 }
 
 // The scan over the chunks, four elements of a unit's state to a thread.  Forward: slot 0 is the initial state (or zero), slot c + 1 =
@@ -173,8 +189,8 @@ __global__ void __launch_bounds__(256) la_scan_kernel(float* __restrict__ states
 }
 
 template <int D> struct OutSmem {
-  float r[64 * (D + PAD)], k[64 * (D + PAD)], S[64 * (D + PAD)], v[64 * LD], A[64 * LD];
-  double L[C];
+  float r[64 * (D + PAD)], k[64 * (D + PAD)], S[D * LD], v[64 * LD], A[64 * LD];      // S: [k][v]
+  Sums L;
 };
 // 64 columns of the outputs of a chunk.
 template <typename T, int D>
@@ -193,7 +209,9 @@ __global__ void __launch_bounds__(NTHR) la_out_kernel(const T* __restrict__ r, c
   load_rows<T, D>(sm.r, LDD, r + base, tok.st, x.rows);
   load_rows<T, D>(sm.k, LDD, k + base, tok.st, x.rows);
   load_rows<T, 64>(sm.v, LD, v + base + 64 * pv, tok.st, x.rows);
-  load_rows<float, D>(sm.S, LDD, states + ((long long)unit * (tok.NT + 1) + c) * (D * D) + 64 * pv * D, D, 64);
+#pragma unroll
+  for (int p = 0; p < D / 64; ++p)
+    load_transposed(sm.S + 64 * p * LD, states + ((long long)unit * (tok.NT + 1) + c) * (D * D) + 64 * pv * D + 64 * p, D);
   __syncthreads();
   const int ig = threadIdx.x >> 4, jg = threadIdx.x & 15;
   float acc[4][4];
@@ -203,14 +221,14 @@ __global__ void __launch_bounds__(NTHR) la_out_kernel(const T* __restrict__ r, c
   for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const int i = ig + 16 * a, j = jg + 16 * b;
-      sm.A[i * LD + j] = j <= i ? acc[a][b] * expf((float)(sm.L[i] - sm.L[j])) : 0.f;
+      const int i = 4 * ig + a, j = jg + 16 * b;
+      sm.A[i * LD + j] = j <= i ? acc[a][b] * expf(between(sm.L, i, j)) : 0.f;
     }
   clear(acc);
-  mm<false, false>(acc, sm.r, LDD, sm.S, LDD, D, ig, jg);
+  mm<false, true>(acc, sm.r, LDD, sm.S, LD, D, ig, jg);
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
-    const float f = expf((float)sm.L[ig + 16 * a]);
+    const float f = expf(sm.L.hi[4 * ig + a]);
 #pragma unroll
     for (int b = 0; b < 4; ++b) acc[a][b] *= f;
   }
@@ -218,18 +236,16 @@ __global__ void __launch_bounds__(NTHR) la_out_kernel(const T* __restrict__ r, c
   mm<false, true>(acc, sm.A, LD, sm.v, LD, 64, ig, jg);
 #pragma unroll
   for (int a = 0; a < 4; ++a) {
-    const int i = ig + 16 * a;
-    if (i < x.rows) {
-#pragma unroll
-      for (int b = 0; b < 4; ++b) o[base + i * tok.st + 64 * pv + jg + 16 * b] = from_f32<T>(acc[a][b]);
-    }
+    const int i = 4 * ig + a;
+    if (i < x.rows) store4(o + base + i * tok.st + 64 * pv + 4 * jg, make_float4(acc[a][0], acc[a][1], acc[a][2], acc[a][3]));
   }
 }
 
 constexpr int G_THR = 2 * NTHR;      // of the gradient kernel
 template <int D> struct GradSmem {
   float r[64 * (D + PAD)], k[64 * (D + PAD)], v[64 * (D + PAD)], d_o[64 * (D + PAD)], A[64 * LD], E[64 * LD], S[2][64 * LD];
-  double L[C], g[C];
+  Sums L;
+  float g[C];
   float pairs[G_THR / 32][C], t1[C], t2[C], t3[G_THR / 32];
 };
 // The sum of x over the 16 threads that hold a row's columns.
@@ -284,8 +300,8 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
   for (int a = 0; a < 4; ++a)
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      const int i = ig + 16 * a, j = jg + 16 * b;
-      (first ? sm.A : sm.E)[i * LD + j] = j <= i ? acc[a][b] * expf((float)(sm.L[i] - sm.L[j])) : 0.f;      // (a choice, so that infinities above the diagonal stay there)
+      const int i = 4 * ig + a, j = jg + 16 * b;
+      (first ? sm.A : sm.E)[i * LD + j] = j <= i ? acc[a][b] * expf(between(sm.L, i, j)) : 0.f;      // (a choice, so that infinities above the diagonal stay there)
     }
   __syncthreads();
   if (!first) {
@@ -293,7 +309,7 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
     for (int a = 0; a < 4; ++a)
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const int i = ig + 16 * a, j = jg + 16 * b;
+        const int i = 4 * ig + a, j = jg + 16 * b;
         sm.S[0][i * LD + j] = j < i ? sm.A[i * LD + j] * acc[a][b] : 0.f;      // (the diagonal does not depend on the decay)
       }
   }
@@ -323,11 +339,11 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
   }
   float f[4];      // the decay between a row's token and the state: before the chunk, behind it
 #pragma unroll
-  for (int a = 0; a < 4; ++a) f[a] = expf((float)(first ? sm.L[ig + 16 * a] : sm.L[C - 1] - sm.L[ig + 16 * a]));
+  for (int a = 0; a < 4; ++a) f[a] = expf(first ? sm.L.hi[4 * ig + a] : between(sm.L, C - 1, 4 * ig + a));
   const int row0 = first ? 0 : 32;      // of dv
   float fv[2];
 #pragma unroll
-  for (int a = 0; a < 2; ++a) fv[a] = expf((float)(sm.L[C - 1] - sm.L[row0 + ig + 16 * a]));
+  for (int a = 0; a < 2; ++a) fv[a] = expf(between(sm.L, C - 1, row0 + 2 * ig + a));
   for (int p = 0; p < P; ++p) {      // 64 columns of each gradient
     clear(acc);
     for (int pv = 0; pv < P; ++pv) {
@@ -340,35 +356,27 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
     const float* q = (first ? sm.r : sm.k) + 64 * p;      // (what it is multiplied with in dg)
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      float s = 0.f;
+      const float4 q4 = *reinterpret_cast<const float4*>(q + (4 * ig + a) * LDD + 4 * jg);
 #pragma unroll
-      for (int b = 0; b < 4; ++b) {
-        acc[a][b] *= f[a];
-        s += acc[a][b] * q[(ig + 16 * a) * LDD + jg + 16 * b];
-      }
-      s = row_sum(s);
-      if (jg == 0) (first ? sm.t1 : sm.t2)[ig + 16 * a] += s;
+      for (int b = 0; b < 4; ++b) acc[a][b] *= f[a];
+      const float s = row_sum(acc[a][0] * q4.x + acc[a][1] * q4.y + acc[a][2] * q4.z + acc[a][3] * q4.w);
+      if (jg == 0) (first ? sm.t1 : sm.t2)[4 * ig + a] += s;
     }
     if (first) mm<false, true>(acc, sm.E, LD, sm.k + 64 * p, LDD, 64, ig, jg);
     else       mm<true, true>(acc, sm.E, LD, sm.r + 64 * p, LDD, 64, ig, jg);
     T* out = first ? dr : dk;
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
-      const int i = ig + 16 * a;
-      if (i < x.rows) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) out[base + i * tok.st + 64 * p + jg + 16 * b] = from_f32<T>(acc[a][b]);
-      }
+      const int i = 4 * ig + a;
+      if (i < x.rows) store4(out + base + i * tok.st + 64 * p + 4 * jg, make_float4(acc[a][0], acc[a][1], acc[a][2], acc[a][3]));
     }
     float av[2][4];
     clear(av);
     for (int pk = 0; pk < P; ++pk) {
-      if (P > 1) {      // (otherwise it is there)
-        __syncthreads();
-        load_rows<float, 64>(sm.S[1], LD, dS + 64 * p * D + 64 * pk, D, 64);
-        __syncthreads();
-      }
-      mm<false, false>(av, sm.k + row0 * LDD + 64 * pk, LDD, sm.S[1], LD, 64, ig, jg);
+      __syncthreads();
+      load_transposed(sm.S[0], dS + 64 * p * D + 64 * pk, D);
+      __syncthreads();
+      mm<false, true>(av, sm.k + row0 * LDD + 64 * pk, LDD, sm.S[0], LD, 64, ig, jg);
     }
 #pragma unroll
     for (int a = 0; a < 2; ++a)
@@ -377,11 +385,8 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
     mm<true, true>(av, sm.A + row0, LD, sm.d_o + 64 * p, LDD, 64, ig, jg);
 #pragma unroll
     for (int a = 0; a < 2; ++a) {
-      const int i = row0 + ig + 16 * a;
-      if (i < x.rows) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) dv[base + i * tok.st + 64 * p + jg + 16 * b] = from_f32<T>(av[a][b]);
-      }
+      const int i = row0 + 2 * ig + a;
+      if (i < x.rows) store4(dv + base + i * tok.st + 64 * p + 4 * jg, make_float4(av[a][0], av[a][1], av[a][2], av[a][3]));
     }
   }
   __syncthreads();
@@ -406,14 +411,14 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
     double t3 = 0.0;
 #pragma unroll
     for (int u = 0; u < NW; ++u) t3 += sm.t3[u];
-    t3 *= exp(sm.L[C - 1]);
+    t3 *= (double)expf(sm.L.hi[C - 1]);
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int i = 2 * lane + q;
       const double dg = pairs[q] + (q ? sa - after[0] : sa) + (q ? sb - before[1] : sb - before[1] - before[0]) + t3;
       if (i < x.rows) {
         const long long at = dw_rows ? (tok.row(x.n) + x.t0 + i) * tok.H + x.h : tok.wbase(x.n, x.h) + (x.t0 + i) * tok.wst;
-        dw[at] = (float)(dg * sm.g[i]);
+        dw[at] = (float)(dg * (double)sm.g[i]);
       }
     }
   }

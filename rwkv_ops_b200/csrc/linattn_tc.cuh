@@ -47,14 +47,13 @@ __device__ __forceinline__ RawW load_w(const Tokens& t, const float* w, long lon
   return x;
 }
 // by one warp; tokens from n on do not decay.  g (may be NULL): the tokens' g
-// (g is a float32 exponential and only its sums are float64: an error of 2^-23 of L, times e^L, is never more than 2^-24.  With exponentials in float64
-// this took 5000 cycles of its warp, for which the others waited.)
+// (with exponentials in float64 this took 5000 cycles of its warp, for which the others waited)
 __device__ __forceinline__ void make_decays(Decays& d, const RawW& x, int n, float* g) {
   const int lane = threadIdx.x & 31;
   float y[4];
   double L[4], s = 0.0;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) y[q] = 4 * lane + q < n ? fmaxf(-expf(x.w[q]), (float)G_FLOOR) : 0.f;
+  for (int q = 0; q < 4; ++q) y[q] = 4 * lane + q < n ? g_of(x.w[q]) : 0.f;
   if (g) *reinterpret_cast<float4*>(g + 4 * lane) = make_float4(y[0], y[1], y[2], y[3]);
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
