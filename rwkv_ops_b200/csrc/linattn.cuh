@@ -30,7 +30,10 @@ namespace la {
 
 // g is a float32 exponential and only its sums are float64: an error of 2^-23 of L, times e^L, is never more than 2^-24.
 constexpr float G_FLOOR = -200.f;
-__device__ __forceinline__ float g_of(float w) { return fmaxf(-expf(w), G_FLOOR); }
+__device__ __forceinline__ float g_of(float w) {
+  const float g = -expf(w);
+  return g < G_FLOOR ? G_FLOOR : g;      // (a NaN stays one)
+}
 
 // Where the tokens lie.  Token tensors have strides sb / st / sh (elements) over batch, token and head, w its own (zero over
 // batch and token where it is a number per head).  Dense: sequence n is batch row n with T tokens; packed (start != nullptr): all

@@ -83,6 +83,18 @@ def test_an_infinity_stays_behind_a_reset_of_another_chunk(dtype):
     assert not torch.isfinite(p[0, 520, 0, 3])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_decay_that_is_not_a_number_is_seen(dtype):
+    import rwkv_ops_b200 as ro
+    x = ref.inputs(1, 400, 2, dtype=dtype, seed=23)
+    a = [x[n].cuda() for n in "rwkv"]
+    o, _ = ro.linear_attention(*a)
+    a[1][0, 300, 1] = math.nan
+    p, s = ro.linear_attention(*a)
+    assert torch.equal(o[:, :256], p[:, :256]) and torch.equal(o[:, :, 0], p[:, :, 0])
+    assert torch.isnan(p[0, 301:, 1]).all() and torch.isnan(s[0, 1]).all()
+
+
 @pytest.mark.parametrize("dtype,D", [(F32, 64), (BF16, 64), (F16, 128)])
 @pytest.mark.parametrize("w,n_state", [("token", 4), ("head", 1)])
 def test_packed(dtype, D, w, n_state):
