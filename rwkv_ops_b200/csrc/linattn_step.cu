@@ -1,13 +1,14 @@
 // Linear attention, one token on a resident state, and the reordering of resident states by beam.
 //
 // Per (sequence, head): S = e^{g} S + v k^T, o = S r, with S [V][K] read and written once: 2 D^2 elements of the state and 4 D of
-// the tokens, so memory is all there is to it (16,384 states of 64 x 64 floats: see the table of times).
+// the tokens, so memory is all there is to it: 16,384 states of 64 x 64 floats in 84 us, 6.5 TB/s, the rate of a copy.  Few states are a launch (32 of them 6.5 us with the call).
 //
 // In a beam search every beam goes on from the state of the beam it was selected from.  A thread owns the same 16 bytes of the
 // states of all beams of a group: it reads them from where the parents are, and writes only after that, so the states are
 // reordered in place, without a second buffer, a barrier or any traffic of its own (a parent of several beams comes from memory
 // once, its other readings from L1).
 #include <algorithm>
+#include <type_traits>
 
 #include "linattn.cuh"
 
@@ -54,12 +55,17 @@ __global__ void __launch_bounds__(STEP_THR) la_step_kernel(const T* __restrict__
   const int g = blockIdx.x / H, h = blockIdx.x % H;
   earlier_kernels_done();
   later_kernels_may_start();
+  // a beam's parent and decay to a lane: found once by a warp, not by every thread
+  const int lane = tid & 31;
+  const long long seq0 = (long long)g * beams;
+  const int from = lane < beams ? parents ? parent_of(parents, seq0 + lane, beams) : lane : 0;
+  const float decay = lane < beams ? decay_of(__ldg(w + (seq0 + lane) * w_stride + h)) : 0.f;
   uint4 X[W][ROWS];
 #pragma unroll
   for (int j = 0; j < W; ++j) {
     if (j < beams) {
-      const long long seq = (long long)g * beams;
-      const int p = parents ? parent_of(parents, seq + j, beams) : j;
+      const long long seq = seq0;
+      const int p = W == 1 ? 0 : __shfl_sync(0xffffffffu, from, j);
       const ST* S = state + ((seq + p) * H + h) * (D * D) + KQ * q;
 #pragma unroll
       for (int x = 0; x < ROWS; ++x) X[j][x] = *reinterpret_cast<const uint4*>(S + (row0 + RG * x) * D);
@@ -68,14 +74,19 @@ __global__ void __launch_bounds__(STEP_THR) la_step_kernel(const T* __restrict__
 #pragma unroll
   for (int j = 0; j < W; ++j) {
     if (j < beams) {
-      const long long seq = (long long)g * beams + j, at = (seq * H + h) * D;
-      const float d = decay_of(__ldg(w + seq * w_stride + h));      // (in float64 this was half the time of a step with beams)
+      const long long seq = seq0 + j, at = (seq * H + h) * D;
+      const float d = __shfl_sync(0xffffffffu, decay, j);
       float rr[KQ], kk[KQ];
+      if constexpr (KQ == 8 && std::is_same<T, __nv_bfloat16>::value) {
+        unpack(__ldg(reinterpret_cast<const uint4*>(r + at + KQ * q)), rr);
+        unpack(__ldg(reinterpret_cast<const uint4*>(k + at + KQ * q)), kk);
+      } else {
 #pragma unroll
-      for (int c = 0; c < KQ; c += 4) {
-        const float4 r4 = load4(r + at + KQ * q + c), k4 = load4(k + at + KQ * q + c);
-        rr[c] = r4.x; rr[c + 1] = r4.y; rr[c + 2] = r4.z; rr[c + 3] = r4.w;
-        kk[c] = k4.x; kk[c + 1] = k4.y; kk[c + 2] = k4.z; kk[c + 3] = k4.w;
+        for (int c = 0; c < KQ; c += 4) {
+          const float4 r4 = load4(r + at + KQ * q + c), k4 = load4(k + at + KQ * q + c);
+          rr[c] = r4.x; rr[c + 1] = r4.y; rr[c + 2] = r4.z; rr[c + 3] = r4.w;
+          kk[c] = k4.x; kk[c + 1] = k4.y; kk[c + 2] = k4.z; kk[c + 3] = k4.w;
+        }
       }
       ST* S = state + (seq * H + h) * (D * D) + KQ * q;
       float sum[ROWS];
