@@ -2,9 +2,10 @@
 // equations are in linattn.cuh; a chunk is 128 tokens, so that products over tokens fill the 128 lanes of TMEM and a thread owns a
 // token's row.
 //
-// Precision.  r, k, v, d_o are bfloat16 and enter products as they are.  Operands that carry a decay are split into hi + lo bfloat16 (two products, 2^-17)
-// wherever the result is a state or a gradient of w, which are float32: the keys (queries) that are added to the state (its gradient), and in the backward both
-// states.  A and E are rounded once to bfloat16, as is the state that meets r in the forward: those results are rounded to bfloat16 anyway.
+// Precision.  r, k, v, d_o are bfloat16 and enter products as they are.  The keys (queries) that are added to the state (its gradient) carry a decay and are split
+// into three bfloat16 parts (three products, exact to float32's last bits: states go from chunk to chunk and are float32).  The states that meet v, k and d_o in the
+// backward are hi + lo (two products, 2^-17): from them come gradients of tokens, and of dw the part that reaches beyond its chunk; room for a third
+// part is not there.  A and E are rounded once to bfloat16, as is the state that meets r in the forward: those results are rounded to bfloat16 anyway.
 //
 // Work is cut into items, a stretch of consecutive chunks of one (sequence, head).  With as many units as the device holds CTAs, an item is a unit.  With
 // fewer, a unit is several parts: a first kernel finds what each adds to the state, keys and values only, and then all parts are walked at once from the state

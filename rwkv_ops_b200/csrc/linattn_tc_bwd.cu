@@ -11,7 +11,7 @@ constexpr int NTHR = 512, NWARP = NTHR / 32;
 
 struct BwdSmem {
   unsigned char r[TOK_BYTES], k[TOK_BYTES], v[TOK_BYTES], d_o[TOK_BYTES];
-  unsigned char rhi[TOK_BYTES], rlo[TOK_BYTES];      // e^{L_i} r_i; dr and dk are staged here afterwards
+  unsigned char rhi[TOK_BYTES], rlo[TOK_BYTES];      // e^{L_i} r_i, of which the third part takes the place of v; dr and dk are staged here afterwards
   unsigned char A[2][TOK_BYTES], E[2][TOK_BYTES];    // [token i][token j], two times 64 columns; dv is staged in the halves that are zero, see stage_v
   unsigned char S[2][TILE_BYTES], dS[2][TILE_BYTES]; // the state before the chunk and the gradient of the one after it, hi and lo, [v][k]
   Decays dec[2];
@@ -22,15 +22,14 @@ struct BwdSmem {
   float near[2][4][4][32], far[2][4][4][32], all[2][4][4];
   float t1[2][4][CT], t2[2][4][CT], t3[2][NWARP];
   uint64_t bar_in, bar_1, bar_x, bar_2;      // rows are here; products are done
-  uint64_t bar_ae, bar_read;                 // of all warps: A and E are stored; r and k have been read
-  uint64_t bar_free, bar_r;                  // the staged gradients have left; the scaled r is stored
+  uint64_t bar_ae, bar_r, bar_read;          // of all warps: A and E are stored; the scaled r is; r and k have been read
+  uint64_t bar_free;                         // the staged gradients have left
   uint32_t tmem_base;
   int sequence;
 };
 // The warps whose block of pairs lies above the diagonal (4, 8, 9, 12, 13, 14) do the other jobs: ISSUE the products (a thread that issues is held up by those
-// under way, some 50 cycles each), STORE the copies of the gradients, DECAYS the next chunk's decays, DW the dw of the chunk before and (LOAD) the loads, and
-// STORE, ISSUE_W and 13 the scaled r.
-constexpr int ISSUE = 14, STORE = 4, DECAYS = 8, LOAD = 12, DW = 12, ISSUE_W = 9, SCALE = 13, SCALE_WARPS = 3;
+// under way, some 50 cycles each), STORE the copies of the gradients, DECAYS the next chunk's decays, DW the dw of the chunk before and (LOAD) the loads.
+constexpr int ISSUE = 14, STORE = 4, DECAYS = 8, LOAD = 12, DW = 12, ISSUE_W = 9;
 constexpr uint32_t TM_S = 0, TM_P = 128, TM_YR = 0, TM_YK = 64, TM_YV = 128, TM_XR = 256, TM_XK = 320, TM_XV = 384, TM_W = 448, TM_COLS = 512;
 
 // the sum over a warp's lanes of x[c], in lanes c and c + 16
@@ -72,8 +71,8 @@ __device__ __forceinline__ void store_split16(unsigned char* hi_t, unsigned char
 // and rows only, and the issuing threads for the warps; all warps meet once, at its end.
 //
 // What bounds it: shared memory.  Operands split into hi and lo, scores, factors and staged gradients are some 767 KB of it a chunk, 6k cycles at 128 bytes each,
-// of the 10k cycles (5.3 us) that a chunk takes; the rest are waits between the batches (tensor pipe 22 % of the cycles, issue slots 41 %).  Measured: B 8 x T 4096,
-// H 32, 357 us for 1.07 GB (3 TB/s); 256 items on 148 SMs are two waves.
+// of the 10k cycles (5.4 us) that a chunk takes; the rest are waits between the batches (tensor pipe 22 % of the cycles, issue slots 41 %).  Measured: B 8 x T 4096,
+// H 32, 361 us for 1.07 GB (3 TB/s); 256 items on 148 SMs are two waves.
 template <bool PACKED>
 __global__ void __launch_bounds__(NTHR, 1)
 la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, const float* __restrict__ states, bf16* __restrict__ dr,
@@ -89,7 +88,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
   const int wq = warp & 3, qt = warp >> 2, row = 32 * wq + lane;
   if (tid == 0) {
     mbar_init(&sm.bar_in, 1); mbar_init(&sm.bar_1, 1); mbar_init(&sm.bar_x, 1); mbar_init(&sm.bar_2, 2);
-    mbar_init(&sm.bar_ae, NWARP); mbar_init(&sm.bar_read, NWARP); mbar_init(&sm.bar_free, 1); mbar_init(&sm.bar_r, SCALE_WARPS);
+    mbar_init(&sm.bar_ae, NWARP); mbar_init(&sm.bar_read, NWARP); mbar_init(&sm.bar_free, 1); mbar_init(&sm.bar_r, NWARP);
     fence_mbar_init();
   }
   if (tid == 32) tma_prefetch_maps(map_r, map_k, map_v, map_do, map_dr, map_dk, map_dv);
@@ -354,40 +353,41 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       }
       tc_fence_before();
       arrive(sm.bar_ae);
-      if (warp == STORE || warp == ISSUE_W || warp == SCALE) {      // the scaled r, 16 bytes of 16 tokens at a time
-        const int first = warp == STORE ? 0 : warp == ISSUE_W ? 48 : 96, n_row = warp == SCALE ? 32 : 48;
-#pragma unroll 2
-        for (int e = lane; e < n_row * 8; e += 64) {
-          uint4 u[2];
-          float f[2];
-          uint32_t off[2];
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int t = first + ((e + 32 * q) >> 3);
-            off[q] = (t >> 6) * TILE_BYTES + tile_chunk_off(t & 63, e & 7);
-            u[q] = *reinterpret_cast<const uint4*>(sm.r + off[q]);
-            f[q] = d.start[t];
-          }
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const uint32_t in[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              const float a = bf16_lo(in[g]) * f[q], b = bf16_hi(in[g]) * f[q];
-              hi[g] = pack_bf16(a, b);
-              lo[g] = pack_bf16(a - bf16_lo(hi[g]), b - bf16_hi(hi[g]));
-            }
-            *reinterpret_cast<uint4*>(sm.rhi + off[q]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(sm.rlo + off[q]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          }
-        }
-        arrive(sm.bar_r);
-      }
-      if (c > x.lo) get_kept(c - 1);
-      // the states' parts of dr and dk, and of dw
+      // the scaled r in three parts, 8 tokens to a warp (B 8 x T 4096, H 32: 361 us; by the three warps that have the least else to do 385; in two parts 357)
+      ok = mbar_wait(&sm.bar_free, ph, status, 518) && ok;
       ok = mbar_wait(&sm.bar_x, ph, status, 514) && ok;
       tc_fence_after();
+      {
+        uint4 u[2];
+        float f[2];
+        uint32_t off[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int t = 8 * warp + 4 * q + (lane >> 3);
+          off[q] = (t >> 6) * TILE_BYTES + tile_chunk_off(t & 63, lane & 7);
+          u[q] = *reinterpret_cast<const uint4*>(sm.r + off[q]);
+          f[q] = d.start[t];
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t in[4] = {u[q].x, u[q].y, u[q].z, u[q].w};
+          uint32_t hi[4], lo[4], rest[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float a = bf16_lo(in[g]) * f[q], b = bf16_hi(in[g]) * f[q];
+            hi[g] = pack_bf16(a, b);
+            a -= bf16_lo(hi[g]); b -= bf16_hi(hi[g]);
+            lo[g] = pack_bf16(a, b);
+            rest[g] = pack_bf16(a - bf16_lo(lo[g]), b - bf16_hi(lo[g]));
+          }
+          *reinterpret_cast<uint4*>(sm.rhi + off[q]) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(sm.rlo + off[q]) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          *reinterpret_cast<uint4*>(sm.v + off[q]) = make_uint4(rest[0], rest[1], rest[2], rest[3]);
+        }
+      }
+      arrive(sm.bar_r);
+      if (c > x.lo) get_kept(c - 1);
+      // the states' parts of dr and dk, and of dw
       const auto state_part = [&](uint32_t col, float f, const unsigned char* tile, float* to) {
         uint32_t a[16];
         float y[16], s = 0.f;
@@ -408,6 +408,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
         if (elect_one()) {
           umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.rhi), false);
           umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.rlo), true);
+          umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.v), true);
           umma_commit(&sm.bar_2);
         }
       }

@@ -13,8 +13,8 @@ constexpr int NTHR = 256;
 constexpr int ISSUE = 5, DECAYS = 4;
 
 struct FwdSmem {
-  unsigned char r[TOK_BYTES], k[TOK_BYTES], v[TOK_BYTES];      // k becomes the hi part of e^{Lc - L_j} k_j
-  unsigned char klo[TOK_BYTES];
+  unsigned char r[TOK_BYTES], k[TOK_BYTES], v[TOK_BYTES];      // k and r become the first and the third part of e^{Lc - L_j} k_j
+  unsigned char klo[TOK_BYTES];       // the second
   unsigned char A[2][TOK_BYTES];      // A [token i][token j], two times 64 columns; the first half stages o afterwards
   unsigned char S[TILE_BYTES];        // the state before the chunk, [v][k], rounded
   Decays dec[2];
@@ -23,7 +23,7 @@ struct FwdSmem {
   int sequence;
 };
 struct AddSmem {      // keys and values alone: three CTAs to an SM
-  unsigned char k[TOK_BYTES], v[TOK_BYTES], klo[TOK_BYTES];
+  unsigned char k[TOK_BYTES], v[TOK_BYTES], klo[TOK_BYTES], r[TOK_BYTES];      // (r: the third part alone)
   Decays dec[2];
   uint64_t bar_in, bar_1, bar_2;
   uint32_t tmem_base;
@@ -40,8 +40,8 @@ constexpr uint32_t TM_S = 0, TM_O2 = 0, TM_O1 = 128;
 // Two CTAs share an SM (113 KB each, 256 TMEM columns each), so that one's products and loads run under the other's arithmetic.
 //
 // What bounds it: the steps of a chunk in turn, products, TMEM reads, the threads' rounding and storing, 3.7 us with two CTAs to an SM (tensor pipe 19 % of the
-// cycles, issue slots 28 %); memory a third below a copy's rate.  Measured, H 32: training of B 8 x T 4096, states kept, 150 us for 671 MB (4.5 TB/s); inference of
-// B 4 x T 16384 343 us, 83 of them in the pass over keys and values, for 1086 MB without that pass.
+// cycles, issue slots 28 %); memory a third below a copy's rate.  Measured, H 32: training of B 8 x T 4096, states kept, 160 us for 671 MB (4.2 TB/s); inference of
+// B 4 x T 16384 384 us, 96 of them in the pass over keys and values, for 1086 MB without that pass.
 template <bool PACKED, bool ADD, bool REV = false>
 __global__ void __launch_bounds__(NTHR, ADD ? 3 : 2)
 la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int n_state, bf16* __restrict__ o, float* __restrict__ ht,
@@ -142,42 +142,48 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
           tc_fence_after();
           umma_tile<128, 128, 0, 0>(tmem_addr(tm, 0, TM_S), smem_u32(sm.r), smem_u32(sm.k), false);
           bulk_wait_read();            // o of the chunk before has left its place in A, which is written to after these products
-          umma_commit(&sm.bar_1);      // (the products with the state run on under what the threads do with these)
           umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_O1), smem_u32(sm.r), smem_u32(sm.S), false);
+          umma_commit(&sm.bar_1);
         }
       }
       if (i + 1 < n_chunks && warp == ISSUE && elect_one()) prefetch_in(chunk(i + 1));
-      // scaled keys, 32 columns of a token; the hi part waits until the products have read the keys as they are
-      uint4 hi[4];
+      // scaled keys, 32 columns of a token, in three parts; two wait until the products have read the keys and queries as they are
+      uint4 hi[4], rest[4];
       {
         const float f = REV ? d.start[row] : d.end[row];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const uint32_t off = (row >> 6) * TILE_BYTES + tile_chunk_off(row & 63, 4 * half + q);
           const uint4 u = *reinterpret_cast<const uint4*>(sm.k + off);
-          uint4 lo;
           const uint32_t in[4] = {u.x, u.y, u.z, u.w};
-          uint32_t h[4], l[4];
+          uint32_t h[4], l[4], m[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float a = bf16_lo(in[e]) * f, b = bf16_hi(in[e]) * f;
+            float a = bf16_lo(in[e]) * f, b = bf16_hi(in[e]) * f;
             h[e] = pack_bf16(a, b);
-            l[e] = pack_bf16(a - bf16_lo(h[e]), b - bf16_hi(h[e]));
+            a -= bf16_lo(h[e]); b -= bf16_hi(h[e]);
+            l[e] = pack_bf16(a, b);
+            m[e] = pack_bf16(a - bf16_lo(l[e]), b - bf16_hi(l[e]));
           }
           hi[q] = make_uint4(h[0], h[1], h[2], h[3]);
-          lo = make_uint4(l[0], l[1], l[2], l[3]);
-          *reinterpret_cast<uint4*>(sm.klo + off) = lo;
+          *reinterpret_cast<uint4*>(sm.klo + off) = make_uint4(l[0], l[1], l[2], l[3]);
+          rest[q] = make_uint4(m[0], m[1], m[2], m[3]);
+          if constexpr (ADD) {      // (no product reads them, and no other thread)
+            *reinterpret_cast<uint4*>(sm.k + off) = hi[q];
+            *reinterpret_cast<uint4*>(sm.r + off) = rest[q];
+          }
         }
       }
       if constexpr (!ADD) {
         ok = mbar_wait(&sm.bar_1, ph, status, 502) && ok;
         tc_fence_after();
-      } else {
-        __syncwarp();
-      }
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<uint4*>(sm.k + (row >> 6) * TILE_BYTES + tile_chunk_off(row & 63, 4 * half + q)) = hi[q];
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t off = (row >> 6) * TILE_BYTES + tile_chunk_off(row & 63, 4 * half + q);
+          *reinterpret_cast<uint4*>(sm.k + off) = hi[q];
+          *reinterpret_cast<uint4*>(sm.r + off) = rest[q];
+        }
+      }
       if constexpr (!ADD) {
         // A: blocks of 32 x 32 on and below the diagonal (warp: rows 32 wq .., columns 64 half ..)
         unsigned char* At = sm.A[half] + (row >> 6) * TILE_BYTES;
@@ -221,6 +227,7 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
         }
         umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.k), false);
         umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.klo), true);
+        umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.r), true);
         umma_commit(&sm.bar_2);
       }
       ok = mbar_wait(&sm.bar_2, ph, status, 503) && ok;
@@ -381,8 +388,8 @@ int launch_pieces(const Args& a, const Cut& cut, const CUtensorMap& map_val, con
                 reverse ? a.tok.n_seq : a.n_state, a.tok.H, cut, (int)reverse);
 }
 
-// How many parts and pieces: the least time by an estimate.  Measured: a chunk takes a CTA 3.9 us where two share an SM, 2.7 alone (backward 5.3, one to an SM), a
-// chunk of the pass over keys and values 2.2 where three do; another launch and what the parts start from 4 us.
+// How many parts and pieces: the least time by an estimate.  Measured: a chunk takes a CTA 4.2 us where two share an SM, 2.8 alone (backward 5.4, one to an SM), a
+// chunk of the pass over keys and values 2.6 where three do; another launch and what the parts start from 4 us.
 Cut cut_units(int n_seq, int max_len, int H, bool backward) {
   constexpr int SMS = 148;      // of a B200
   const int NT = (max_len + CT - 1) / CT, units = n_seq * H, slots = backward ? SMS : 2 * SMS;
@@ -396,7 +403,7 @@ Cut cut_units(int n_seq, int max_len, int H, bool backward) {
     c.sub = (c.per + c.per_sub - 1) / c.per_sub;
     const long long items = (long long)units * parts;
     const double waves = (double)((items + slots - 1) / slots);
-    const double t = waves * c.per * (backward ? 5.3 : items > SMS ? 3.9 : 2.7) + (parts > 1 ? 4 + 2.2 * c.per_sub : 0);
+    const double t = waves * c.per * (backward ? 5.4 : items > SMS ? 4.2 : 2.8) + (parts > 1 ? 4 + 2.6 * c.per_sub : 0);
     if (t < least) { least = t; best = c; }
   }
   return best;
