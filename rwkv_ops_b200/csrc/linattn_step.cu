@@ -98,7 +98,10 @@ __global__ void __launch_bounds__(STEP_THR) la_step_kernel(const T* __restrict__
         sum[x] = 0.f;
 #pragma unroll
         for (int c = 0; c < KQ; ++c) {
-          s[c] = fmaf(s[c], d, vv * kk[c]);
+          // a state that is rounded to bfloat16: the two products and the sum as written, so that it is bit for bit what this arithmetic gives anywhere (a
+          // difference in float32's last place can become one in bfloat16's, which the states after it keep)
+          if constexpr (KQ == 8) s[c] = __fadd_rn(__fmul_rn(s[c], d), __fmul_rn(vv, kk[c]));
+          else s[c] = fmaf(s[c], d, vv * kk[c]);
           sum[x] = fmaf(s[c], rr[c], sum[x]);      // (from the float32 value of the new state, whatever it is stored as)
         }
         *reinterpret_cast<uint4*>(S + (row0 + RG * x) * D) = pack(s);

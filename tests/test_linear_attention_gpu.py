@@ -314,6 +314,29 @@ def test_steps_are_the_operator(D, dtype, state_dtype, w):
     assert float((dec.final_state().double().cpu() - s).norm() / s.norm()) <= tol
 
 
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_a_bfloat16_state_is_that_of_float32_arithmetic(dtype, D):
+    """Bit for bit, over the steps of an answer (without a decay: its exponential is not the same everywhere)."""
+    import rwkv_ops_b200 as ro
+    B, T, H = 2, 12, 3
+    x = ref.inputs(B, T, H, D, dtype=dtype, n_state=B, seed=24)
+    dec = ro.LinearAttentionDecodeState(B, H, head_size=D, state_dtype=BF16, initial_state=x["s0"].cuda())
+    S = x["s0"].to(BF16)
+    none = torch.full((H,), -1e9)
+    for t in range(T):
+        r, k, v = (x[n][:, t].float() for n in "rkv")
+        S = S.float() * 1.0 + v[..., :, None] * k[..., None, :]
+        o = (S.double() * r[..., None, :].double()).sum(-1)
+        size = (S.double() * r[..., None, :].double()).abs().sum(-1)
+        S = S.to(BF16)
+        got = dec.step(x["r"][:, t].cuda(), none.cuda(), x["k"][:, t].cuda(), x["v"][:, t].cuda())
+        assert torch.equal(dec.state.cpu(), S), t
+        # D products added in float32, at most D roundings of at most the sum of their sizes; and a rounding to the type
+        off = (got.double().cpu() - o).abs() - torch.finfo(dtype).eps / 2 * o.abs()
+        assert bool((off <= D * 2.0 ** -24 * size).all()), t
+
+
 @pytest.mark.parametrize("state_dtype", [F32, BF16])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("groups,beams", [(3, 1), (2, 2), (4, 3), (2, 5), (1, 8), (2, 11), (1, 32)])
