@@ -48,9 +48,8 @@ size_t rwkvb200_linattn_states_bytes(int n_seq, int max_len, int H, int head_siz
 
 size_t rwkvb200_linattn_workspace_bytes(int n_seq, int max_len, int total, int H, int head_size, int dtype, int w_per_head, int backward) {
   if (check_dims(n_seq, max_len, H, head_size, dtype)) return 0;
-  const long long rows = total > 0 ? total : (long long)n_seq * max_len;
   if (la::tc_applies(head_size, dtype)) return la::tc_scratch_bytes(n_seq, max_len, H, w_per_head, backward);
-  return la::simt_scratch_bytes(n_seq, max_len, H, head_size, rows, w_per_head, backward);
+  return la::simt_scratch_bytes(n_seq, max_len, H, head_size, w_per_head, backward);
 }
 
 int rwkvb200_linattn_fwd(const void* r, const float* w, int w_per_head, const void* k, const void* v, const float* h0, int n_state, void* o,
@@ -69,7 +68,7 @@ int rwkvb200_linattn_fwd(const void* r, const float* w, int w_per_head, const vo
   a.r = r; a.k = k; a.v = v; a.w = w; a.h0 = n_state ? h0 : nullptr; a.n_state = n_state;
   a.o = o; a.ht = ht; a.states = states; a.scratch = workspace;
   a.w_per_head = w_per_head != 0; a.dtype = dtype; a.D = head_size;
-  a.w_rows = seq_start ? total : (long long)n_seq * max_len;
+  a.tokens = seq_start ? total : (long long)n_seq * max_len;
   a.tok = tokens_of(seq_start, seq_len, n_seq, max_len, total, H, head_size, head_first, w_per_head);
   return la::tc_applies(head_size, dtype) ? la::launch_tc_fwd(a, (cudaStream_t)stream) : la::launch_simt_fwd(a, (cudaStream_t)stream);
 }
@@ -89,7 +88,7 @@ int rwkvb200_linattn_bwd(const void* r, const float* w, int w_per_head, const vo
   a.r = r; a.k = k; a.v = v; a.w = w; a.d_o = d_o; a.d_ht = d_ht;
   a.dr = dr; a.dw = dw; a.dk = dk; a.dv = dv; a.dh0 = dh0; a.states = const_cast<float*>(states); a.scratch = workspace;
   a.w_per_head = w_per_head != 0; a.dtype = dtype; a.D = head_size;
-  a.w_rows = seq_start ? total : (long long)n_seq * max_len;
+  a.tokens = seq_start ? total : (long long)n_seq * max_len;
   a.tok = tokens_of(seq_start, seq_len, n_seq, max_len, total, H, head_size, head_first, w_per_head);
   return la::tc_applies(head_size, dtype) ? la::launch_tc_bwd(a, (cudaStream_t)stream) : la::launch_simt_bwd(a, (cudaStream_t)stream);
 }

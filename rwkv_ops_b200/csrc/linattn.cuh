@@ -46,8 +46,6 @@ struct Tokens {
   __device__ __forceinline__ int length(int n) const { return len ? __ldg(len + n) : T; }
   __device__ __forceinline__ long long base(int n, int h) const { return (start ? __ldg(start + n) * st : n * sb) + h * sh; }
   __device__ __forceinline__ long long wbase(int n, int h) const { return (start ? __ldg(start + n) * wst : n * wsb) + h * wsh; }
-  // the place of a token in a [tokens][H] float32 array (the gradient of w before it is summed)
-  __device__ __forceinline__ long long row(int n) const { return start ? (long long)__ldg(start + n) : (long long)n * T; }
 };
 
 // What a call works on; pointers that do not apply are NULL.
@@ -60,19 +58,19 @@ struct Args {
   float* states;          // [n_seq * H][chunks][D][D]: the state before every chunk (linattn_simt.cu: and the last one)
   void* scratch;
   int n_state, w_per_head, dtype, D;
-  long long w_rows;       // tokens in all (rows of a [tokens][H] array)
+  long long tokens;       // in all
   Tokens tok;
 };
 
-// The gradient of a w per head: partial sums [parts][H] in float64, added up in a fixed order.
-int launch_sum_dw(const float* dw_tok, long long rows, int H, double* partial, float* dw, cudaStream_t st);
+// The gradient of a w per head, from what stretches of sequences add to it [rows][H]: partial sums [parts][H] in float64, added up in a fixed order.
+int launch_sum_dw(const float* dw_rows, long long rows, int H, double* partial, float* dw, cudaStream_t st);
 constexpr int DW_PARTS = 128;
 
 // float32 arithmetic on the CUDA cores: every dtype, head sizes 64 and 128, chunks of 64 tokens (linattn_simt.cu)
 int launch_simt_fwd(const Args& a, cudaStream_t st);
 int launch_simt_bwd(const Args& a, cudaStream_t st);
 size_t simt_states_bytes(int n_seq, int max_len, int H, int D);
-size_t simt_scratch_bytes(int n_seq, int max_len, int H, int D, long long rows, bool w_per_head, bool backward);
+size_t simt_scratch_bytes(int n_seq, int max_len, int H, int D, bool w_per_head, bool backward);
 
 // tensor cores: bfloat16 tokens, head size 64, chunks of 128 tokens (linattn_tc_fwd.cu, linattn_tc_bwd.cu)
 inline bool tc_applies(int D, int dtype) { return D == 64 && dtype == RWKVB200_BF16; }

@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
                                                         const float* __restrict__ w, const T* __restrict__ d_o,
                                                         const float* __restrict__ states, const float* __restrict__ dstates,
                                                         T* __restrict__ dr, T* __restrict__ dk, T* __restrict__ dv, float* __restrict__ dw,
-                                                        int dw_rows, Tokens tok) {
+                                                        int dw_parts, Tokens tok) {
   extern __shared__ __align__(16) unsigned char raw[];
   GradSmem<D>& sm = *reinterpret_cast<GradSmem<D>*>(raw);
   constexpr int LDD = D + PAD, P = D / 64, NW = G_THR / 32;
@@ -275,7 +275,11 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
   later_kernels_may_start();
   const int c = blockIdx.x % tok.NT, unit = blockIdx.x / tok.NT, tid = threadIdx.x;
   const Where x = where(tok, unit, c);
-  if (c >= x.NT) return;
+  const long long part = ((long long)x.n * tok.NT + c) * tok.H + x.h;      // of a w per head: what this chunk adds to its gradient
+  if (c >= x.NT) {
+    if (dw_parts && tid == 0) dw[part] = 0.f;
+    return;
+  }
   prefix(sm.L, sm.g, tok, w, tok.wbase(x.n, x.h), x.t0, x.rows);
   const long long base = tok.base(x.n, x.h) + x.t0 * tok.st;
   load_rows<T, D>(sm.r, LDD, r + base, tok.st, x.rows);
@@ -417,14 +421,21 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
 #pragma unroll
     for (int u = 0; u < NW; ++u) t3 += sm.t3[u];
     t3 *= (double)expf(sm.L.hi[C - 1]);
+    double sum = 0.0;
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int i = 2 * lane + q;
       const double dg = pairs[q] + (q ? sa - after[0] : sa) + (q ? sb - before[1] : sb - before[1] - before[0]) + t3;
       if (i < x.rows) {
-        const long long at = dw_rows ? (tok.row(x.n) + x.t0 + i) * tok.H + x.h : tok.wbase(x.n, x.h) + (x.t0 + i) * tok.wst;
-        dw[at] = (float)(dg * (double)sm.g[i]);
+        const double y = dg * (double)sm.g[i];
+        if (dw_parts) sum += y;
+        else dw[tok.wbase(x.n, x.h) + (x.t0 + i) * tok.wst] = (float)y;
       }
+    }
+    if (dw_parts) {
+#pragma unroll
+      for (int m = 16; m >= 1; m >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+      if (lane == 0) dw[part] = (float)sum;
     }
   }
 }
@@ -463,7 +474,7 @@ __global__ void __launch_bounds__(256) la_dw_sum_kernel(const double* __restrict
 inline size_t a256(size_t x) { return (x + 255) & ~size_t(255); }
 
 struct Scratch { float *dstates, *decay, *dw; double* part; };
-Scratch scratch_of(void* p, const Tokens& t, int D, long long rows, bool w_per_head, bool backward) {
+Scratch scratch_of(void* p, const Tokens& t, int D, bool w_per_head, bool backward) {
   Scratch s = {};
   unsigned char* q = static_cast<unsigned char*>(p);
   const size_t units = (size_t)t.n_seq * t.H;
@@ -471,7 +482,7 @@ Scratch scratch_of(void* p, const Tokens& t, int D, long long rows, bool w_per_h
   if (backward) {
     s.dstates = reinterpret_cast<float*>(q); q += a256(units * (t.NT + 1) * D * D * 4);
     if (w_per_head) {
-      s.dw = reinterpret_cast<float*>(q); q += a256((size_t)rows * t.H * 4);
+      s.dw = reinterpret_cast<float*>(q); q += a256(units * t.NT * 4);      // [n_seq][chunks][H]
       s.part = reinterpret_cast<double*>(q);
     }
   }
@@ -482,7 +493,7 @@ template <typename T, int D>
 int fwd(const Args& a, cudaStream_t st) {
   const Tokens& t = a.tok;
   const int units = t.n_seq * t.H;
-  const Scratch s = scratch_of(a.scratch, t, D, a.w_rows, a.w_per_head, false);
+  const Scratch s = scratch_of(a.scratch, t, D, a.w_per_head, false);
   DeviceFacts f;
   if (int e = device_facts(&f)) return e;
   {
@@ -506,7 +517,7 @@ template <typename T, int D>
 int bwd(const Args& a, cudaStream_t st) {
   const Tokens& t = a.tok;
   const int units = t.n_seq * t.H;
-  const Scratch s = scratch_of(a.scratch, t, D, a.w_rows, a.w_per_head, true);
+  const Scratch s = scratch_of(a.scratch, t, D, a.w_per_head, true);
   DeviceFacts f;
   if (int e = device_facts(&f)) return e;
   {
@@ -525,27 +536,27 @@ int bwd(const Args& a, cudaStream_t st) {
     if (int e = launch(la_grad_kernel<T, D>, t.NT * units, G_THR, smem, st, 1, (const T*)a.r, (const T*)a.k, (const T*)a.v, a.w, (const T*)a.d_o,
                        (const float*)a.states, (const float*)s.dstates, (T*)a.dr, (T*)a.dk, (T*)a.dv, a.w_per_head ? s.dw : a.dw, a.w_per_head, t)) return e;
   }
-  return a.w_per_head ? launch_sum_dw(s.dw, a.w_rows, t.H, s.part, a.dw, st) : RWKVB200_OK;
+  return a.w_per_head ? launch_sum_dw(s.dw, (long long)t.n_seq * t.NT, t.H, s.part, a.dw, st) : RWKVB200_OK;
 }
 
 }  // namespace
 
-int launch_sum_dw(const float* dw_tok, long long rows, int H, double* partial, float* dw, cudaStream_t st) {
+int launch_sum_dw(const float* dw_rows, long long rows, int H, double* partial, float* dw, cudaStream_t st) {
   ProfScope prof("linattn_dw_kernel", st);
   const int parts = (int)(rows < DW_PARTS * 8 ? (rows + 7) / 8 : DW_PARTS);
-  if (int e = launch(la_dw_part_kernel, dim3(parts, (H + 31) / 32), 256, 0, st, 1, dw_tok, rows, H, partial)) return e;
+  if (int e = launch(la_dw_part_kernel, dim3(parts, (H + 31) / 32), 256, 0, st, 1, dw_rows, rows, H, partial)) return e;
   return launch(la_dw_sum_kernel, (H + 7) / 8, 256, 0, st, 1, (const double*)partial, parts, H, dw);
 }
 
 size_t simt_states_bytes(int n_seq, int max_len, int H, int D) {
   return (size_t)n_seq * H * ((max_len + C - 1) / C + 1) * D * D * 4;
 }
-size_t simt_scratch_bytes(int n_seq, int max_len, int H, int D, long long rows, bool w_per_head, bool backward) {
+size_t simt_scratch_bytes(int n_seq, int max_len, int H, int D, bool w_per_head, bool backward) {
   const size_t units = (size_t)n_seq * H, NT = (max_len + C - 1) / C;
   size_t n = a256(units * NT * 4);
   if (backward) {
     n += a256(units * (NT + 1) * D * D * 4);
-    if (w_per_head) n += a256((size_t)rows * H * 4) + a256((size_t)DW_PARTS * H * 8);
+    if (w_per_head) n += a256(units * NT * 4) + a256((size_t)DW_PARTS * H * 8);
   }
   return n;
 }

@@ -489,7 +489,7 @@ int bwd(const Args& a, cudaStream_t st) {
   static_assert(smem <= 227 * 1024, "one CTA to an SM");
   if (int e = need_aligned_smem<la_tc_bwd_kernel<PACKED>>(f)) return e;
   if (int e = allow_smem<la_tc_bwd_kernel<PACKED>>(f, smem)) return e;
-  const int B = t.start ? 1 : t.n_seq, T = t.start ? (int)a.w_rows : t.T, head_first = t.st == 64 && t.H > 1;
+  const int B = t.start ? 1 : t.n_seq, T = t.start ? (int)a.tokens : t.T, head_first = t.st == 64 && t.H > 1;
   const void* in[] = {a.r, a.k, a.v, a.d_o, a.dr, a.dk, a.dv};
   CUtensorMap m[7];
   for (int i = 0; i < 7; ++i)

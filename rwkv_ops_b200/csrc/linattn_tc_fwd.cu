@@ -347,7 +347,7 @@ int fwd(const Args& a, cudaStream_t st) {
   static_assert(smem <= 115712, "two CTAs of 113 KB each share an SM");
   if (int e = need_aligned_smem<la_tc_fwd_kernel<PACKED, false>>(f)) return e;
   if (int e = allow_smem<la_tc_fwd_kernel<PACKED, false>>(f, smem)) return e;
-  const int B = t.start ? 1 : t.n_seq, T = t.start ? (int)a.w_rows : t.T, head_first = t.st == 64 && t.H > 1;
+  const int B = t.start ? 1 : t.n_seq, T = t.start ? (int)a.tokens : t.T, head_first = t.st == 64 && t.H > 1;
   CUtensorMap mr, mk, mv, mo;
   const void* r = a.r ? a.r : a.k;      // (the states alone: whatever r k^T is, it goes nowhere)
   if (int e = make_token_tensor_map(&mr, r, B, T, t.H, head_first)) return e;
