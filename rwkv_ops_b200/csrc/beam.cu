@@ -4,14 +4,14 @@
 //   candidate (i, t) has the score s_i + x_i[t] - log sum_u e^{x_i[u]};   the W best, ties to the lowest i V + t.
 //
 // What bounds it is reading the logits once.  The W best of a row come from its own logits in their own order.  A warp streams a slice of a row and
-// keeps, for each lane, the running maximum, the tile it is in, the largest of the other tiles and the running sum: some 150 instructions for 512 tokens, where
+// keeps, for each lane, the running maximum, the tile it is in, the largest of the other tiles and the running sum: some 250 instructions for 512 tokens, where
 // sorted lists kept on the way took three times that in time.  The W-th largest of the lanes' maxima is at most the W-th best of the row, so only the lanes that
 // reach it have any of the W best: a few of the row's lanes, of which 16 tokens each (all, where another tile reaches it, too) are read once more, from L2, and
 // offered to a list.  One cluster of CTAs works on a group; its warps' lists and sums meet in the shared memory of the first CTA, where the normalisers are put
 // together and candidates compared in float64: a sum of two float32 would tie where the scores do not.
 // What runs once is kept short in code: it is fetched while everyone waits for it.
-// Measured: 64 groups of 8 beams over 50277 float32 logits 36 us, 2.9 TB/s: the stream near memory's rate, then second look, lists and merging, one after the other,
-// each a wait on shared memory or L2 (issue slots 46 %, most stalls at barriers).  One group of 4 beams over 65536 bfloat16 logits 12.3 us with the call.
+// Measured: 64 groups of 8 beams over 50277 float32 logits 35 us, 2.9 TB/s: the stream near memory's rate, then second look, lists and merging, one after the other,
+// each a wait on shared memory or L2 (issue slots 46 %, most stalls at barriers).  One group of 4 beams over 65536 bfloat16 logits 12.9 us with the call.
 //
 // A beam that has finished goes on with `eos` alone, at the score it has; its logits are not read.  NaN and +inf logits count as -inf (never
 // generated), a NaN score as -inf.  Where fewer than W candidates are possible the rest are impossible ones, score -inf, lowest
@@ -31,6 +31,7 @@ constexpr int NWARP = 16;      // of a CTA
 constexpr int MAXC = 8;        // CTAs of a cluster
 constexpr int MAXW = 32;
 constexpr float NEG = -INFINITY;
+constexpr float LN2 = 0.6931471805599453f, LOG2E_LO = (float)(1.4426950408889634 - (double)tc::LOG2E);
 
 // A list of the best (value, index) of a warp, sorted, entry l in lane l; entries beyond the first `n` lanes do not matter.
 template <typename F, typename I>
@@ -120,17 +121,37 @@ struct Tile {
   }
 };
 
-// Running maximum and sum of a lane, in float32: a lane adds a few hundred terms that are at most one.
+// Running maximum of a lane, and the sum of e^{x - ref} over its tokens.  A row that has few warps gives a lane thousands of terms (V / 32 with one warp), so the sum
+// is two floats, s + c: a tile's 16 terms are added pair by pair and go in with what rounding loses kept in c; one float32 dropped every faint term behind a large one
+// (2e-4 of the logarithm at 131072 tokens).  `ref` follows the maximum only when that is 8 above it: each move multiplies the sum by a rounded factor, and a sum
+// that matters sees two of them at most.  A term is 2^y (1 + ln 2 r), y = d log2 e as rounded and r what the rounding left out, some 2^-24 |d|: without r, a million
+// equal faint tokens are off by the same amount each.
 struct Sum {
-  float m = NEG, s = 0.f;
-  template <int N> __device__ __forceinline__ void add(const float (&x)[N], float top) {
-    if (top > m) {
-      s *= tc::ex2((m - top) * tc::LOG2E);      // (m = -inf: the factor is zero)
-      m = top;
+  float m = NEG, ref = NEG, s = 0.f, c = 0.f;
+  __device__ __forceinline__ void add(const float (&x)[16], float top) {
+    if (top > m) m = top;
+    if (top > ref + 8.f) {
+      const float f = expf(ref - top);      // (ref = -inf: zero)
+      s *= f;
+      c *= f;
+      ref = top;
     }
-    const float base = m == NEG ? 0.f : m;
+    const float base = ref == NEG ? 0.f : ref;
+    float four[4], r = 0.f;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += tc::ex2((x[i] - base) * tc::LOG2E);
+    for (int q = 0; q < 4; ++q) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float d = fmaxf(x[4 * q + i] - base, -200.f), y = d * tc::LOG2E;      // (2^-288: zero)
+        e[i] = tc::ex2(y);
+        r = fmaf(e[i], fmaf(d, LOG2E_LO, fmaf(d, tc::LOG2E, -y)), r);
+      }
+      four[q] = (e[0] + e[1]) + (e[2] + e[3]);
+    }
+    const float p = (four[0] + four[1]) + (four[2] + four[3]), t = s + p, b = t - s;
+    c += fmaf(LN2, r, (s - (t - b)) + (p - b));
+    s = t;
   }
 };
 
@@ -146,7 +167,8 @@ struct Smem {
     struct { double score[MAXW * MAXW + MAXW]; long long at[MAXW * MAXW + MAXW]; } last;      // then the group's candidates
   };
   Key best[MAXW][MAXW];                            // of a row: its W best
-  float m[MAXC * NWARP], s[MAXC * NWARP];          // of every warp of the cluster
+  double s[MAXC * NWARP];                          // of every warp of the cluster: the sum relative to its maximum
+  float m[MAXC * NWARP];                           // and that
   double top[MAXW], shift[MAXW];                   // of a row: the maximum; s_i - log (sum relative to it)
   float top_lanes[NWARP][MAXW];                    // of this CTA's warps, the W largest of the lanes' maxima
 };
@@ -199,14 +221,12 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
   int at = lo;            // that tile
   if (lo < hi) {
     const bool words = (reinterpret_cast<uintptr_t>(x) & 3) == 0;
-    Tile<T> next[2];      // the next tiles are on their way while one is looked at
-    next[0].load(x, lo * TILE, V, lane, words);
-    if (lo + 1 < hi) next[1].load(x, (lo + 1) * TILE, V, lane, words);
+    Tile<T> next;      // the next tile is on its way while one is looked at (two of them cost spilled registers: 64 groups of 8 float32 rows 47.6 us, so 35.0)
+    next.load(x, lo * TILE, V, lane, words);
 #pragma unroll 1
     for (int t = lo; t < hi; ++t) {
-      const Tile<T> tile = next[0];
-      next[0] = next[1];
-      if (t + 2 < hi) next[1].load(x, (t + 2) * TILE, V, lane, words);
+      const Tile<T> tile = next;
+      if (t + 1 < hi) next.load(x, (t + 1) * TILE, V, lane, words);
       float f[16];
       tile.values(f);
       float top = f[0];
@@ -269,14 +289,14 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
   float m = sum.m;
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  float s = sum.m == NEG ? 0.f : sum.s * tc::ex2((sum.m - m) * tc::LOG2E);
+  double s = sum.m == NEG ? 0.0 : ((double)sum.s + (double)sum.c) * (double)expf(sum.ref - m);
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
   cluster_wait();
   const uint32_t home = tc::cluster_addr(tc::smem_u32(&sm), 0);
   auto put = [&](const void* p, int bits) {      // a word to the first CTA
     tc::store_cluster(home + (tc::smem_u32(p) - tc::smem_u32(&sm)), bits); };
-  if (lane == 0) { put(&sm.m[all], __float_as_int(m)); put(&sm.s[all], __float_as_int(s)); }
+  if (lane == 0) { put(&sm.m[all], __float_as_int(m)); put(&sm.s[all], __double2loint(s)); put(reinterpret_cast<const int*>(&sm.s[all]) + 1, __double2hiint(s)); }
   if (lane < W) {
     const uint32_t* k = reinterpret_cast<const uint32_t*>(&sm.key[all * W + lane]);
     const bool any = best.i != RowBest::NONE;
@@ -298,7 +318,7 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
     double ss = 0.0;
     for (int q = lane; q < per_row; q += 32) {
       const float mq = sm.m[i * per_row + q];
-      if (mq != NEG) ss += (double)(sm.s[i * per_row + q] * tc::ex2((mq - mm) * tc::LOG2E));
+      if (mq != NEG) ss += sm.s[i * per_row + q] * (double)expf(mq - mm);
     }
 #pragma unroll
     for (int d = 16; d >= 1; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
