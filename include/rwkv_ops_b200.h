@@ -340,6 +340,10 @@ int rwkvb200_wkv6_bwd_varlen(const void* r, const void* k, const void* v, const 
  *   h0           float32 [n_state][H][D][D], n_state 0 (none: zero), 1 (shared) or n_seq;  ht [n_seq][H][D][D], may be NULL
  *   states       rwkvb200_linattn_states_bytes(..., keep = 1) of memory in which the forward leaves the states that the backward starts from; a
  *                forward without a backward passes keep = 0 and that much (possibly none).  o NULL: the states alone.
+ *                A packed batch whose sequences lie in the order of their places, none overlapping another, needs no more than
+ *                rwkvb200_linattn_packed_states_bytes and rwkvb200_linattn_packed_workspace_bytes: the chunks of its tokens and one more to a
+ *                sequence, where the functions above count those of the longest sequence for each.  states_bytes says which: below
+ *                rwkvb200_linattn_states_bytes(..., keep = 1) the states lie compactly.  The backward gets the forward's states_bytes.
  * Backward: gradients of r, w (like w, float32), k, v and of the state each sequence started from (dh0 [n_seq][H][D][D], may be NULL);
  * d_ht may be NULL (zero).  workspace: rwkvb200_linattn_workspace_bytes (total 0 for a dense batch).
  * rwkvb200_linattn_step: one token in place on resident states [groups * beams][H][D][D], float32 or bfloat16; with parents
@@ -349,6 +353,8 @@ int rwkvb200_wkv6_bwd_varlen(const void* r, const void* k, const void* v, const 
  * ---------------------------------------------------------------------------------------- */
 size_t rwkvb200_linattn_states_bytes(int n_seq, int max_len, int H, int head_size, int dtype, int keep);
 size_t rwkvb200_linattn_workspace_bytes(int n_seq, int max_len, int total, int H, int head_size, int dtype, int w_per_head, int backward);
+size_t rwkvb200_linattn_packed_states_bytes(int n_seq, int max_len, int total, int H, int head_size, int dtype, int keep);
+size_t rwkvb200_linattn_packed_workspace_bytes(int n_seq, int max_len, int total, int H, int head_size, int dtype, int w_per_head, int backward);
 int rwkvb200_linattn_fwd(const void* r, const float* w, int w_per_head, const void* k, const void* v,
                          const float* h0, int n_state, void* o, float* ht, float* states, size_t states_bytes,
                          void* workspace, size_t workspace_bytes, const int32_t* seq_start, const int32_t* seq_len,

@@ -60,6 +60,8 @@ SIGNATURES = {
                                  [_I] * 4 + [_P]),
     "rwkvb200_linattn_states_bytes": (c_size_t, [_I] * 6),
     "rwkvb200_linattn_workspace_bytes": (c_size_t, [_I] * 8),
+    "rwkvb200_linattn_packed_states_bytes": (c_size_t, [_I] * 7),
+    "rwkvb200_linattn_packed_workspace_bytes": (c_size_t, [_I] * 8),
     "rwkvb200_linattn_fwd": (c_int, [_P, _P, _I, _P, _P, _P, _I, _P, _P, _P, _Z, _P, _Z, _P, _P] + [_I] * 7 + [_P]),
     "rwkvb200_linattn_bwd": (c_int, [_P, _P, _I] + [_P] * 5 + [_Z] + [_P] * 6 + [_Z, _P, _P] + [_I] * 7 + [_P]),
     "rwkvb200_linattn_step": (c_int, [_P, _P, _I, _P, _P, _P, _I, _P, _P] + [_I] * 5 + [_P]),
@@ -156,11 +158,17 @@ def wkv6_kept_bytes(B: int, T: int, H: int) -> int:
             + _a256(B * H * 4) + _a256(B * H * 64 * 64 * 4) + _a256((B * H + 1) * 4))
 
 
-def linattn_states_bytes(n_seq: int, max_len: int, H: int, D: int, dtype: torch.dtype) -> int:
-    """Likewise for ``rwkvb200_linattn_states_bytes(..., keep = 1)``: the states of linear attention before chunks of 128 tokens on the
-    tensor-core path (bfloat16, head size 64), before and after chunks of 64 elsewhere."""
-    chunks = (max_len + 127) // 128 if D == 64 and dtype == torch.bfloat16 else (max_len + 63) // 64 + 1
-    return n_seq * H * chunks * D * D * 4
+def linattn_states_bytes(n_seq: int, max_len: int, H: int, D: int, dtype: torch.dtype, total: int | None = None) -> int:
+    """Likewise for ``rwkvb200_linattn_states_bytes(..., keep = 1)``, or with ``total`` for ``rwkvb200_linattn_packed_states_bytes``: the states
+    of linear attention before chunks of 128 tokens on the tensor-core path (bfloat16, head size 64), before and after chunks of 64
+    elsewhere.  A packed batch has the chunks of its tokens and one more to a sequence, or those of the longest sequence for each, if
+    that is less."""
+    tc = D == 64 and dtype == torch.bfloat16
+    C, more = (128, 0) if tc else (64, 1)
+    chunks = n_seq * ((max_len + C - 1) // C)
+    if total is not None:
+        chunks = torch.sym_min(chunks, total // C + n_seq)
+    return (chunks + more * n_seq) * H * D * D * 4
 
 
 def strerror(code: int) -> str:

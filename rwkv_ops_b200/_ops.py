@@ -122,8 +122,8 @@ def _register_fakes():
     @fake("rwkv_ops_b200::linattn_fwd")
     def _(r, w, k, v, seq_start, seq_len, max_len, h0, head_first, keep):
         B, T, H, D = dims(r, head_first)
-        n, length = (B, T) if seq_start is None else (seq_start.numel(), max_len)
-        return torch.empty_like(r), state(r, n, H, D), kept(r, _lib.linattn_states_bytes(n, length, H, D, r.dtype) if keep else 0)
+        n, length, total = (B, T, None) if seq_start is None else (seq_start.numel(), max_len, T)
+        return torch.empty_like(r), state(r, n, H, D), kept(r, _lib.linattn_states_bytes(n, length, H, D, r.dtype, total) if keep else 0)
 
     @fake("rwkv_ops_b200::linattn_bwd")
     def _(r, w, k, v, seq_start, seq_len, max_len, h0, d_o, d_ht, k_, head_first):

@@ -23,6 +23,8 @@
 // stay finite.
 #pragma once
 
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace rwkvb200 {
@@ -42,11 +44,28 @@ struct Tokens {
   long long sb, st, sh, wsb, wst, wsh;
   const int* start;
   const int* len;
-  int n_seq, T, H, NT;      // NT: chunk slots of a sequence
+  int n_seq, T, H;
+  // What is kept of every chunk of C = 2^shift tokens lies in slots.  Dense: NT of them to a (sequence, head), as many as the longest sequence has chunks.  Packed and compact:
+  // `slots` of them to a head, sequence n's from start[n] / C + n on; sequences in the order of their places, none overlapping another, never meet there (a
+  // sequence has at most len / C + 1 chunks), and one long sequence among many short ones takes what its tokens take and not their number times its length.
+  int shift, NT, slots, compact;
   __device__ __forceinline__ int length(int n) const { return len ? __ldg(len + n) : T; }
   __device__ __forceinline__ long long base(int n, int h) const { return (start ? __ldg(start + n) * st : n * sb) + h * sh; }
   __device__ __forceinline__ long long wbase(int n, int h) const { return (start ? __ldg(start + n) * wst : n * wsb) + h * wsh; }
+  // the first slot of a (sequence, head); with one slot more than chunks to a sequence where `more` is 1
+  __device__ __forceinline__ int place(int n, int more) const { return (__ldg(start + n) >> shift) + n * (1 + more); }
+  __device__ __forceinline__ long long first(int n, int h, int more) const {
+    return compact ? (long long)h * (slots + more * n_seq) + place(n, more) : (long long)(n * H + h) * (NT + more);
+  }
 };
+
+// Chunk slots of a head (dense and padded: of all its sequences), and whether they are compact: where that is fewer.
+inline long long padded_slots(int n_seq, int max_len, int C) { return (long long)n_seq * ((max_len + (long long)C - 1) / C); }
+inline long long compact_slots(int n_seq, int total, int C) { return total / C + (long long)n_seq; }
+inline long long chunk_slots(int n_seq, int max_len, int total, int C) {      // total 0: not compact
+  const long long p = padded_slots(n_seq, max_len, C);
+  return total > 0 ? std::min(p, compact_slots(n_seq, total, C)) : p;
+}
 
 // What a call works on; pointers that do not apply are NULL.
 struct Args {
@@ -55,12 +74,19 @@ struct Args {
   void *o, *dr, *dk, *dv;
   float *ht, *dh0;
   float* dw;              // gradient of w: like w
-  float* states;          // [n_seq * H][chunks][D][D]: the state before every chunk (linattn_simt.cu: and the last one)
+  float* states;          // [slots][D][D]: the state before every chunk (linattn_simt.cu: and the last one)
   void* scratch;
-  int n_state, w_per_head, dtype, D;
+  int n_state, w_per_head, dtype, D, compact;
   long long tokens;       // in all
   Tokens tok;
 };
+
+// The chunks of a call's tokens, C (64 or 128) of them to a chunk.
+inline void set_chunks(Args& a, int C) {
+  Tokens& t = a.tok;
+  t.shift = C == 128 ? 7 : 6; t.NT = (int)((t.T + (long long)C - 1) / C); t.compact = a.compact;
+  t.slots = (int)chunk_slots(t.n_seq, t.T, a.compact ? (int)a.tokens : 0, C);
+}
 
 // The gradient of a w per head, from what stretches of sequences add to it [rows][H]: partial sums [parts][H] in float64, added up in a fixed order.
 int launch_sum_dw(const float* dw_rows, long long rows, int H, double* partial, float* dw, cudaStream_t st);
@@ -69,14 +95,14 @@ constexpr int DW_PARTS = 128;
 // float32 arithmetic on the CUDA cores: every dtype, head sizes 64 and 128, chunks of 64 tokens (linattn_simt.cu)
 int launch_simt_fwd(const Args& a, cudaStream_t st);
 int launch_simt_bwd(const Args& a, cudaStream_t st);
-size_t simt_states_bytes(int n_seq, int max_len, int H, int D);
-size_t simt_scratch_bytes(int n_seq, int max_len, int H, int D, bool w_per_head, bool backward);
+size_t simt_states_bytes(int n_seq, int max_len, int total, int H, int D);      // total 0: dense or padded
+size_t simt_scratch_bytes(int n_seq, int max_len, int total, int H, int D, bool w_per_head, bool backward);
 
 // tensor cores: bfloat16 tokens, head size 64, chunks of 128 tokens (linattn_tc_fwd.cu, linattn_tc_bwd.cu)
 inline bool tc_applies(int D, int dtype) { return D == 64 && dtype == RWKVB200_BF16; }
 int launch_tc_fwd(const Args& a, cudaStream_t st);
 int launch_tc_bwd(const Args& a, cudaStream_t st);
-size_t tc_states_bytes(int n_seq, int max_len, int H, bool keep);
+size_t tc_states_bytes(int n_seq, int max_len, int total, int H, bool keep);
 size_t tc_scratch_bytes(int n_seq, int max_len, int H, bool w_per_head, bool backward);
 
 // one token in place on states [groups * beams][H][D][D], float32 or bfloat16 (linattn_step.cu); w_stride: H, or 0 for a w per head

@@ -108,29 +108,53 @@ __device__ __forceinline__ void prefix(Sums& L, float* g, const Tokens& t, const
   }
 }
 
-struct Where { int n, h, unit, len, NT, t0, rows; };
-__device__ __forceinline__ Where where(const Tokens& t, int unit, int c) {
+// The sequence of a packed batch that slot s belongs to: the last one whose slots start at s or before, found by a warp, 32 of them at a time (one look for 32
+// sequences, two for 1024); -1: s is before the first.
+__device__ __forceinline__ int sequence_of(const Tokens& t, int s) {
+  const int lane = threadIdx.x & 31;
+  int lo = -1, end = t.n_seq;
+  while (end - lo > 1) {      // it is lo or one of lo + 1 .. end - 1
+    const int step = (end - lo - 1 + 31) / 32, at = lo + 1 + lane * step;
+    const int n = __popc(__ballot_sync(0xffffffffu, at < end && t.place(at, 0) <= s));
+    const int from = lo;
+    if (n) lo = from + 1 + (n - 1) * step;
+    end = min(end, from + 1 + n * step);
+    if (!n) end = from + 1;
+  }
+  return lo;
+}
+// Which chunk a block works on: chunk c of (sequence n, head h), none where rows < 1.  `slot`: of the head's, over all sequences.
+struct Where { int n, h, c, slot, t0, rows; };
+__device__ __forceinline__ Where where(const Tokens& t) {
   Where x;
-  x.unit = unit; x.n = unit / t.H; x.h = unit % t.H;
-  x.len = t.length(x.n);
-  x.NT = (x.len + C - 1) / C;
-  x.t0 = c * C;
-  x.rows = min(C, x.len - x.t0);
+  const int b = blockIdx.x;
+  if (t.compact) {
+    x.h = b / t.slots; x.slot = b % t.slots;
+    x.n = sequence_of(t, x.slot);
+    x.c = x.n < 0 ? 0 : x.slot - t.place(x.n, 0);
+  } else {
+    const int unit = b / t.NT;
+    x.c = b % t.NT;
+    x.n = unit / t.H; x.h = unit % t.H;
+    x.slot = x.n * t.NT + x.c;
+  }
+  x.t0 = x.c * C;
+  x.rows = x.n < 0 ? 0 : min(C, t.length(x.n) - x.t0);
   return x;
 }
 
 // What a chunk adds to the state (REV: to its gradient, walking backwards), a 64 x 64 block of it, into the slot after (before) the chunk, and the
 // chunk's decay.
 template <typename T, int D, bool REV>
-__global__ void __launch_bounds__(NTHR) la_add_kernel(const T* __restrict__ val, const T* __restrict__ key, const float* __restrict__ w,
+__global__ void __launch_bounds__(NTHR, 4) la_add_kernel(const T* __restrict__ val, const T* __restrict__ key, const float* __restrict__ w,
                                                       float* __restrict__ states, float* __restrict__ decay, Tokens tok) {
   __shared__ __align__(16) float av[64 * LD], bk[64 * LD];
   __shared__ Sums L;
   earlier_kernels_done();
   later_kernels_may_start();
-  const int c = blockIdx.x % tok.NT, unit = blockIdx.x / tok.NT, pv = blockIdx.y / (D / 64), pk = blockIdx.y % (D / 64);
-  const Where x = where(tok, unit, c);
-  if (c >= x.NT) return;
+  const int pv = blockIdx.y / (D / 64), pk = blockIdx.y % (D / 64);
+  const Where x = where(tok);
+  if (x.rows < 1) return;
   prefix(L, nullptr, tok, w, tok.wbase(x.n, x.h), x.t0, x.rows);
   const long long base = tok.base(x.n, x.h) + x.t0 * tok.st;
   load_rows<T, 64>(av, LD, val + base + 64 * pv, tok.st, x.rows);
@@ -145,10 +169,10 @@ __global__ void __launch_bounds__(NTHR) la_add_kernel(const T* __restrict__ val,
   float acc[4][4];
   clear(acc);
   mm<true, true>(acc, av, LD, bk, LD, 64, ig, jg);
-  float* out = states + ((long long)unit * (tok.NT + 1) + (REV ? c : c + 1)) * (D * D) + (64 * pv) * D + 64 * pk;
+  float* out = states + (tok.first(x.n, x.h, 1) + (REV ? x.c : x.c + 1)) * (D * D) + (64 * pv) * D + 64 * pk;
 #pragma unroll
   for (int a = 0; a < 4; ++a) store4(out + (4 * ig + a) * D + 4 * jg, make_float4(acc[a][0], acc[a][1], acc[a][2], acc[a][3]));
-  if (blockIdx.y == 0 && threadIdx.x == 0) decay[(long long)unit * tok.NT + c] = expf(L.hi[C - 1]);
+  if (blockIdx.y == 0 && threadIdx.x == 0) decay[tok.first(x.n, x.h, 0) + x.c] = expf(L.hi[C - 1]);
 }
 
 // The scan over the chunks, four elements of a unit's state to a thread.  Forward: slot 0 is the initial state (or zero), slot c + 1 =
@@ -164,8 +188,8 @@ __global__ void __launch_bounds__(256) la_scan_kernel(float* __restrict__ states
   const int n = unit / tok.H, h = unit % tok.H, NT = (tok.length(n) + C - 1) / C;
   float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
   if (first && n_first > 0) S = *reinterpret_cast<const float4*>(first + ((long long)(n_first == 1 ? 0 : n) * tok.H + h) * (D * D) + e);
-  float* slot = states + (long long)unit * (tok.NT + 1) * (D * D) + e;
-  const float* dec = decay + (long long)unit * tok.NT;
+  float* slot = states + tok.first(n, h, 1) * (D * D) + e;
+  const float* dec = decay + tok.first(n, h, 0);
   *reinterpret_cast<float4*>(slot + (long long)(REV ? NT : 0) * (D * D)) = S;
   constexpr int AHEAD = 8;
   for (int c0 = 0; c0 < NT; c0 += AHEAD) {
@@ -205,9 +229,9 @@ __global__ void __launch_bounds__(NTHR) la_out_kernel(const T* __restrict__ r, c
   constexpr int LDD = D + PAD;
   earlier_kernels_done();
   later_kernels_may_start();
-  const int c = blockIdx.x % tok.NT, unit = blockIdx.x / tok.NT, pv = blockIdx.y;
-  const Where x = where(tok, unit, c);
-  if (c >= x.NT) return;
+  const int pv = blockIdx.y;
+  const Where x = where(tok);
+  if (x.rows < 1) return;
   prefix(sm.L, nullptr, tok, w, tok.wbase(x.n, x.h), x.t0, x.rows);
   const long long base = tok.base(x.n, x.h) + x.t0 * tok.st;
   load_rows<T, D>(sm.r, LDD, r + base, tok.st, x.rows);
@@ -215,7 +239,7 @@ __global__ void __launch_bounds__(NTHR) la_out_kernel(const T* __restrict__ r, c
   load_rows<T, 64>(sm.v, LD, v + base + 64 * pv, tok.st, x.rows);
 #pragma unroll
   for (int p = 0; p < D / 64; ++p)
-    load_transposed(sm.S + 64 * p * LD, states + ((long long)unit * (tok.NT + 1) + c) * (D * D) + 64 * pv * D + 64 * p, D);
+    load_transposed(sm.S + 64 * p * LD, states + (tok.first(x.n, x.h, 1) + x.c) * (D * D) + 64 * pv * D + 64 * p, D);
   __syncthreads();
   const int ig = threadIdx.x >> 4, jg = threadIdx.x & 15;
   float acc[4][4];
@@ -273,10 +297,10 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
   constexpr int LDD = D + PAD, P = D / 64, NW = G_THR / 32;
   earlier_kernels_done();
   later_kernels_may_start();
-  const int c = blockIdx.x % tok.NT, unit = blockIdx.x / tok.NT, tid = threadIdx.x;
-  const Where x = where(tok, unit, c);
-  const long long part = ((long long)x.n * tok.NT + c) * tok.H + x.h;      // of a w per head: what this chunk adds to its gradient
-  if (c >= x.NT) {
+  const int tid = threadIdx.x;
+  const Where x = where(tok);
+  const long long part = (long long)x.slot * tok.H + x.h;      // of a w per head: what this chunk adds to its gradient
+  if (x.rows < 1) {
     if (dw_parts && tid == 0) dw[part] = 0.f;
     return;
   }
@@ -286,8 +310,8 @@ __global__ void __launch_bounds__(G_THR) la_grad_kernel(const T* __restrict__ r,
   load_rows<T, D>(sm.k, LDD, k + base, tok.st, x.rows);
   load_rows<T, D>(sm.v, LDD, v + base, tok.st, x.rows);
   load_rows<T, D>(sm.d_o, LDD, d_o + base, tok.st, x.rows);
-  const float* S0 = states + ((long long)unit * (tok.NT + 1) + c) * (D * D);
-  const float* dS = dstates + ((long long)unit * (tok.NT + 1) + c + 1) * (D * D);
+  const float* S0 = states + (tok.first(x.n, x.h, 1) + x.c) * (D * D);
+  const float* dS = dstates + (tok.first(x.n, x.h, 1) + x.c + 1) * (D * D);
   const bool first = tid < NTHR;      // which half
   const int ig = (tid & (NTHR - 1)) >> 4, jg = tid & 15, warp = tid >> 5, lane = tid & 31;
   // <dS, S0>
@@ -477,12 +501,12 @@ struct Scratch { float *dstates, *decay, *dw; double* part; };
 Scratch scratch_of(void* p, const Tokens& t, int D, bool w_per_head, bool backward) {
   Scratch s = {};
   unsigned char* q = static_cast<unsigned char*>(p);
-  const size_t units = (size_t)t.n_seq * t.H;
-  s.decay = reinterpret_cast<float*>(q); q += a256(units * t.NT * 4);
+  const size_t slots = (size_t)t.slots * t.H, more = (size_t)t.n_seq * t.H;
+  s.decay = reinterpret_cast<float*>(q); q += a256(slots * 4);
   if (backward) {
-    s.dstates = reinterpret_cast<float*>(q); q += a256(units * (t.NT + 1) * D * D * 4);
+    s.dstates = reinterpret_cast<float*>(q); q += a256((slots + more) * D * D * 4);
     if (w_per_head) {
-      s.dw = reinterpret_cast<float*>(q); q += a256(units * t.NT * 4);      // [n_seq][chunks][H]
+      s.dw = reinterpret_cast<float*>(q); q += a256(slots * 4);      // [slots][H]
       s.part = reinterpret_cast<double*>(q);
     }
   }
@@ -498,7 +522,7 @@ int fwd(const Args& a, cudaStream_t st) {
   if (int e = device_facts(&f)) return e;
   {
     ProfScope prof("linattn_add_kernel", st);
-    if (int e = launch(la_add_kernel<T, D, false>, dim3(t.NT * units, D * D / 4096), NTHR, 0, st, 1, (const T*)a.v, (const T*)a.k, a.w, a.states,
+    if (int e = launch(la_add_kernel<T, D, false>, dim3(t.slots * t.H, D * D / 4096), NTHR, 0, st, 1, (const T*)a.v, (const T*)a.k, a.w, a.states,
                        s.decay, t)) return e;
   }
   {
@@ -509,7 +533,7 @@ int fwd(const Args& a, cudaStream_t st) {
   ProfScope prof("linattn_out_kernel", st);
   constexpr int smem = (int)sizeof(OutSmem<D>);
   if (int e = allow_smem<la_out_kernel<T, D>>(f, smem)) return e;
-  return launch(la_out_kernel<T, D>, dim3(t.NT * units, D / 64), NTHR, smem, st, 1, (const T*)a.r, (const T*)a.k, (const T*)a.v, a.w,
+  return launch(la_out_kernel<T, D>, dim3(t.slots * t.H, D / 64), NTHR, smem, st, 1, (const T*)a.r, (const T*)a.k, (const T*)a.v, a.w,
                 (const float*)a.states, (T*)a.o, t);
 }
 
@@ -522,7 +546,7 @@ int bwd(const Args& a, cudaStream_t st) {
   if (int e = device_facts(&f)) return e;
   {
     ProfScope prof("linattn_add_kernel", st);
-    if (int e = launch(la_add_kernel<T, D, true>, dim3(t.NT * units, D * D / 4096), NTHR, 0, st, 1, (const T*)a.d_o, (const T*)a.r, a.w, s.dstates,
+    if (int e = launch(la_add_kernel<T, D, true>, dim3(t.slots * t.H, D * D / 4096), NTHR, 0, st, 1, (const T*)a.d_o, (const T*)a.r, a.w, s.dstates,
                        s.decay, t)) return e;
   }
   {
@@ -533,10 +557,10 @@ int bwd(const Args& a, cudaStream_t st) {
     ProfScope prof("linattn_grad_kernel", st);
     constexpr int smem = (int)sizeof(GradSmem<D>);
     if (int e = allow_smem<la_grad_kernel<T, D>>(f, smem)) return e;
-    if (int e = launch(la_grad_kernel<T, D>, t.NT * units, G_THR, smem, st, 1, (const T*)a.r, (const T*)a.k, (const T*)a.v, a.w, (const T*)a.d_o,
+    if (int e = launch(la_grad_kernel<T, D>, t.slots * t.H, G_THR, smem, st, 1, (const T*)a.r, (const T*)a.k, (const T*)a.v, a.w, (const T*)a.d_o,
                        (const float*)a.states, (const float*)s.dstates, (T*)a.dr, (T*)a.dk, (T*)a.dv, a.w_per_head ? s.dw : a.dw, a.w_per_head, t)) return e;
   }
-  return a.w_per_head ? launch_sum_dw(s.dw, (long long)t.n_seq * t.NT, t.H, s.part, a.dw, st) : RWKVB200_OK;
+  return a.w_per_head ? launch_sum_dw(s.dw, t.slots, t.H, s.part, a.dw, st) : RWKVB200_OK;
 }
 
 }  // namespace
@@ -548,24 +572,28 @@ int launch_sum_dw(const float* dw_rows, long long rows, int H, double* partial, 
   return launch(la_dw_sum_kernel, (H + 7) / 8, 256, 0, st, 1, (const double*)partial, parts, H, dw);
 }
 
-size_t simt_states_bytes(int n_seq, int max_len, int H, int D) {
-  return (size_t)n_seq * H * ((max_len + C - 1) / C + 1) * D * D * 4;
+size_t simt_states_bytes(int n_seq, int max_len, int total, int H, int D) {
+  return (size_t)(chunk_slots(n_seq, max_len, total, C) + n_seq) * H * D * D * 4;
 }
-size_t simt_scratch_bytes(int n_seq, int max_len, int H, int D, bool w_per_head, bool backward) {
-  const size_t units = (size_t)n_seq * H, NT = (max_len + C - 1) / C;
-  size_t n = a256(units * NT * 4);
+size_t simt_scratch_bytes(int n_seq, int max_len, int total, int H, int D, bool w_per_head, bool backward) {
+  const size_t slots = (size_t)chunk_slots(n_seq, max_len, total, C) * H;
+  size_t n = a256(slots * 4);
   if (backward) {
-    n += a256(units * (NT + 1) * D * D * 4);
-    if (w_per_head) n += a256(units * NT * 4) + a256((size_t)DW_PARTS * H * 8);
+    n += a256((slots + (size_t)n_seq * H) * D * D * 4);
+    if (w_per_head) n += a256(slots * 4) + a256((size_t)DW_PARTS * H * 8);
   }
   return n;
 }
 
-int launch_simt_fwd(const Args& a, cudaStream_t st) {
+int launch_simt_fwd(const Args& args, cudaStream_t st) {
+  Args a = args;
+  set_chunks(a, C);
   RWKVB200_DISPATCH_DTYPE(a.dtype, return a.D == 64 ? fwd<T, 64>(a, st) : fwd<T, 128>(a, st));
   return RWKVB200_OK;
 }
-int launch_simt_bwd(const Args& a, cudaStream_t st) {
+int launch_simt_bwd(const Args& args, cudaStream_t st) {
+  Args a = args;
+  set_chunks(a, C);
   RWKVB200_DISPATCH_DTYPE(a.dtype, return a.D == 64 ? bwd<T, 64>(a, st) : bwd<T, 128>(a, st));
   return RWKVB200_OK;
 }

@@ -114,6 +114,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       tma_load_4d(sm.v + q * TILE_BYTES, &map_v, &sm.bar_in, 0, t0 + 64 * q, x.h, brow);
     }
   };
+  auto kept_slot = [&](int c) { return PACKED ? tok.first(x.n, x.h, 0) + c : (long long)x.unit * tok.NT + c; };
   auto prefetch_in = [&](int c) {
     const int t0 = seq0 + c * CT;
 #pragma unroll
@@ -123,7 +124,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       tma_prefetch_4d(&map_do, 0, t0 + 64 * q, x.h, brow);
       tma_prefetch_4d(&map_v, 0, t0 + 64 * q, x.h, brow);
     }
-    bulk_prefetch_l2(states + ((long long)x.unit * tok.NT + c) * 4096, 4096 * 4);
+    bulk_prefetch_l2(states + kept_slot(c) * 4096, 4096 * 4);
   };
   auto stage_v = [&](int tile) { return tile ? sm.E[1] : sm.A[1]; };      // 64 rows of dv: rows 0 .. 63 of the right halves, all above the diagonal
   auto store_out = [&](int c) {      // the staged gradients of a chunk
@@ -151,7 +152,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
   const long long sat = (long long)srow * 64 + 16 * qt;
   float dS[16], S0[16];
   auto get_kept = [&](int c) {
-    const float* from = states + ((long long)x.unit * tok.NT + c) * 4096;
+    const float* from = states + kept_slot(c) * 4096;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float4 f = st_lane ? __ldcg(reinterpret_cast<const float4*>(from + kept_at(4 * qt + j, wq, lane))) : make_float4(0.f, 0.f, 0.f, 0.f);
@@ -517,7 +518,7 @@ int bwd(const Args& a, cudaStream_t st) {
 
 int launch_tc_bwd(const Args& a, cudaStream_t st) {
   Args b = a;
-  b.tok.NT = (a.tok.T + CT - 1) / CT;
+  set_chunks(b, CT);
   return a.tok.start ? bwd<true>(b, st) : bwd<false>(b, st);
 }
 

@@ -104,7 +104,7 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
 #pragma unroll
     for (int j = 0; j < 8; ++j) *reinterpret_cast<float4*>(to + kept_at(8 * half + j, wq, lane)) = make_float4(S[4 * j], S[4 * j + 1], S[4 * j + 2], S[4 * j + 3]);
   };
-  auto keep_state = [&](int c) { put_kept(states + ((long long)x.unit * tok.NT + c) * 4096); };
+  auto keep_state = [&](int c) { put_kept(states + (PACKED ? tok.first(x.n, x.h, 0) + c : (long long)x.unit * tok.NT + c) * 4096); };
   bool ok = true;
   float product = 1.f;
   const int n_chunks = x.hi - x.lo;
@@ -409,8 +409,8 @@ Cut cut_units(int n_seq, int max_len, int H, bool backward) {
   return best;
 }
 
-size_t tc_states_bytes(int n_seq, int max_len, int H, bool keep) {
-  return keep ? (size_t)n_seq * H * ((max_len + CT - 1) / CT) * 4096 * 4 : 0;
+size_t tc_states_bytes(int n_seq, int max_len, int total, int H, bool keep) {
+  return keep ? (size_t)chunk_slots(n_seq, max_len, total, CT) * H * 4096 * 4 : 0;
 }
 
 size_t tc_scratch_bytes(int n_seq, int max_len, int H, bool w_per_head, bool backward) {
@@ -422,7 +422,7 @@ size_t tc_scratch_bytes(int n_seq, int max_len, int H, bool w_per_head, bool bac
 
 int launch_tc_fwd(const Args& a, cudaStream_t st) {
   Args b = a;
-  b.tok.NT = (a.tok.T + CT - 1) / CT;
+  set_chunks(b, CT);
   return a.tok.start ? fwd<true>(b, st) : fwd<false>(b, st);
 }
 

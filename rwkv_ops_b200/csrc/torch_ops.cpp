@@ -763,12 +763,21 @@ LaDims linattn_dims(const Tensor& r, const OptTensor& seq_start, int64_t max_len
   if (has(seq_start)) return {(int)seq_start->numel(), (int)max_len, d.T, d.H, d.K};
   return {d.B, d.T, 0, d.H, d.K};
 }
+// Memory for the states and for a call's workspace; packed sequences lie in the order of their places, so that their chunks are stored compactly.
+size_t linattn_states_bytes(const LaDims& d, int code, bool keep) {
+  return d.total ? rwkvb200_linattn_packed_states_bytes(d.n_seq, d.max_len, d.total, d.H, d.D, code, keep)
+                 : rwkvb200_linattn_states_bytes(d.n_seq, d.max_len, d.H, d.D, code, keep);
+}
+size_t linattn_workspace_bytes(const LaDims& d, int code, bool per_head, bool backward) {
+  return d.total ? rwkvb200_linattn_packed_workspace_bytes(d.n_seq, d.max_len, d.total, d.H, d.D, code, per_head, backward)
+                 : rwkvb200_linattn_workspace_bytes(d.n_seq, d.max_len, 0, d.H, d.D, code, per_head, backward);
+}
 // the states between chunks into `states` (undefined: none are left), and o, ht where they are defined
 void linattn_forward(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const OptTensor& seq_start, const OptTensor& seq_len,
                      const LaDims& d, const OptTensor& h0, bool head_first, const Tensor& o, const Tensor& ht, const Tensor& kept) {
   const int code = dtype_code(r.scalar_type()), per_head = w.dim() == 1;
-  const size_t ns = rwkvb200_linattn_states_bytes(d.n_seq, d.max_len, d.H, d.D, code, kept.defined());
-  const size_t nw = rwkvb200_linattn_workspace_bytes(d.n_seq, d.max_len, d.total, d.H, d.D, code, per_head, 0);
+  const size_t ns = linattn_states_bytes(d, code, kept.defined());
+  const size_t nw = linattn_workspace_bytes(d, code, per_head, false);
   const Tensor states = kept.defined() ? kept : ns ? bytes(ns, r) : Tensor(), ws = nw ? bytes(nw, r) : Tensor();
   check(rwkvb200_linattn_fwd(ptr(r), fptr(w), per_head, ptr(k), ptr(v), fptr(h0), n_state_of(h0), ptr(o), fptr(ht), fptr(states), ns, ptr(ws), nw,
                              iptr(seq_start), iptr(seq_len), d.n_seq, d.max_len, d.total, d.H, d.D, code, head_first, stream_of(r)),
@@ -780,7 +789,7 @@ Three linattn_fwd(const Tensor& r, const Tensor& w, const Tensor& k, const Tenso
   const c10::cuda::CUDAGuard guard(r.device());
   const LaDims d = linattn_dims(r, seq_start, max_len, head_first);
   Tensor o = fresh_like(r), ht = fresh({d.n_seq, d.H, d.D, d.D}, at::kFloat, r), kept;
-  if (keep) kept = bytes(rwkvb200_linattn_states_bytes(d.n_seq, d.max_len, d.H, d.D, dtype_code(r.scalar_type()), 1), r);
+  if (keep) kept = bytes(linattn_states_bytes(d, dtype_code(r.scalar_type()), true), r);
   linattn_forward(r, w, k, v, seq_start, seq_len, d, h0, head_first, o, ht, kept);
   return {o, ht, keep ? kept : bytes(0, r)};
 }
@@ -792,8 +801,8 @@ Five linattn_bwd(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor
   const LaDims d = linattn_dims(r, seq_start, max_len, head_first);
   const int code = dtype_code(r.scalar_type()), per_head = w.dim() == 1;
   Tensor dr = fresh_like(r), dw = fresh_like(w), dk = fresh_like(r), dv = fresh_like(r), dh0 = fresh({d.n_seq, d.H, d.D, d.D}, at::kFloat, r);
-  const size_t ns = rwkvb200_linattn_states_bytes(d.n_seq, d.max_len, d.H, d.D, code, 1);
-  const size_t nw = rwkvb200_linattn_workspace_bytes(d.n_seq, d.max_len, d.total, d.H, d.D, code, per_head, 1);
+  const size_t ns = linattn_states_bytes(d, code, true);
+  const size_t nw = linattn_workspace_bytes(d, code, per_head, true);
   Tensor states = kept;
   if ((size_t)kept.numel() < ns) {
     states = bytes(ns, r);
@@ -861,9 +870,12 @@ std::tuple<Tensor, Tensor> linear_attention(const Tensor& r, const Tensor& w, co
   if (any_requires_grad({&r_, &w_, &k_, &v_}, h0)) {
     const auto limit = (int64_t)std::min<size_t>(keep_limit_bytes(r.device().index()), std::numeric_limits<int64_t>::max());
     const SymInt len = packed ? SymInt(max_len) : d.T;
-    // (rwkvb200_linattn_states_bytes, of sizes that may be symbols)
-    const SymInt chunks = d.K == HEAD && t == at::kBFloat16 ? (len + 127) / 128 : (len + 63) / 64 + 1;
-    keep = TORCH_STATICALLY_KNOWN_TRUE((n_seq * d.H * chunks * d.K * d.K * 4).sym_le(limit));
+    // (rwkvb200_linattn_states_bytes and _packed_states_bytes, of sizes that may be symbols; the latter is the lesser of two)
+    const bool tc = d.K == HEAD && t == at::kBFloat16;
+    const int64_t c = tc ? 128 : 64, more = tc ? 0 : 1;
+    const SymInt state = d.H * d.K * d.K * 4;
+    keep = TORCH_STATICALLY_KNOWN_TRUE((n_seq * ((len + (c - 1)) / c + more) * state).sym_le(limit)) ||
+           (packed && TORCH_STATICALLY_KNOWN_TRUE(((d.T / c + n_seq * (1 + more)) * state).sym_le(limit)));
   }
   auto [o, ht, kept] = RWKV_OP(linattn_fwd, "linattn_fwd", r_, w_, k_, v_, seq_start, seq_len, max_len, h0, head_first, keep);
   return {o.to(r.scalar_type()), ht};

@@ -28,12 +28,19 @@ def sequences_alone(x, start, lens, n_state):
 
 @pytest.mark.parametrize("dtype,D", [(F32, 64), (BF16, 64), (F16, 64), (F32, 128), (BF16, 128)])
 @pytest.mark.parametrize("w", ["head", "token"])
-def test_rows_of_no_sequence(dtype, D, w):
+@pytest.mark.parametrize("start,lens,total,compact", [
+    ([3, 140, 161, 300], [130, 1, 64, 200], 517, False),
+    ([300, 161, 3, 140], [200, 64, 130, 1], 517, False),                           # in any order
+    ([3, 700, 705, 706, 771], [650, 3, 1, 64, 129], 920, True),                    # the chunks' states one behind another
+    ([0, 1, 2, 3, 4, 5, 6], [1, 1, 1, 1, 1, 1, 514], 520, True),
+    ([128 + 2 * i for i in range(40)] + [250], [1 + i % 2 for i in range(40)] + [300], 550, True),      # (more than a warp looks through at once)
+])
+def test_rows_of_no_sequence(dtype, D, w, start, lens, total, compact):
     """Rows before, between and behind the sequences: whatever they and the workspace hold (NaN), nothing of it reaches a result, and no
     output is written there."""
     from rwkv_ops_b200 import _lib
     lib = _lib.load()
-    start, lens, total, H, code = [3, 140, 161, 300], [130, 1, 64, 200], 517, 3, CODE[dtype]
+    H, code = 3, CODE[dtype]
     n = len(lens)
     x = ref.inputs(1, total, H, D, dtype=dtype, w=w, seed=31)
     g = torch.Generator().manual_seed(32)
@@ -57,8 +64,14 @@ def test_rows_of_no_sequence(dtype, D, w):
     p = lambda t: t.data_ptr()
     per_head, longest = int(w == "head"), max(lens)
     sizes = (n, longest, total, H, D, code)
-    states = nan(lib.rwkvb200_linattn_states_bytes(n, longest, H, D, code, 1))
-    ws = [nan(lib.rwkvb200_linattn_workspace_bytes(*sizes, per_head, backward)) for backward in (0, 1)]
+    if compact:
+        need, padded = lib.rwkvb200_linattn_packed_states_bytes(*sizes, 1), lib.rwkvb200_linattn_states_bytes(n, longest, H, D, code, 1)
+        assert need < padded
+        states = nan(need)
+        ws = [nan(lib.rwkvb200_linattn_packed_workspace_bytes(*sizes, per_head, backward)) for backward in (0, 1)]
+    else:
+        states = nan(lib.rwkvb200_linattn_states_bytes(n, longest, H, D, code, 1))
+        ws = [nan(lib.rwkvb200_linattn_workspace_bytes(*sizes, per_head, backward)) for backward in (0, 1)]
     stream = torch.cuda.current_stream().cuda_stream
     assert lib.rwkvb200_linattn_fwd(p(a["r"]), p(a["w"]), per_head, p(a["k"]), p(a["v"]), p(s0), n, p(out["o"]), p(out["s"]), p(states), states.numel(),
                                     p(ws[0]), ws[0].numel(), p(at), p(ln), n, longest, total, H, D, code, 0, stream) == 0
@@ -69,3 +82,38 @@ def test_rows_of_no_sequence(dtype, D, w):
         assert (out[q][:, outside.cuda()] == SENTINEL).all(), q
         out[q] = out[q][:, rows.cuda()]
     ref.check(out, want, dtype)
+
+
+@pytest.mark.parametrize("dtype,D,w,n_short", [(BF16, 64, "head", 300), (BF16, 64, "token", 700), (F32, 64, "head", 300), (F16, 64, "token", 1100),
+                                               (BF16, 128, "head", 40)])
+@pytest.mark.parametrize("keep", [True, False])
+def test_one_long_sequence_among_many_short_ones(dtype, D, w, n_short, keep, monkeypatch):
+    """What a packed batch is, and that it takes the memory of its tokens: states of some 64 or 128 tokens each and one or two more to a sequence, not the
+    longest sequence's for every one."""
+    import rwkv_ops_b200 as ro
+    if not keep:
+        monkeypatch.setenv("RWKV_OPS_B200_KEEP_LIMIT_MB", "0")
+    g = torch.Generator().manual_seed(33)
+    H = 2
+    lens = torch.randint(1, 12, (n_short,), generator=g).tolist()
+    lens[n_short // 3] = 1500 if D == 64 else 700
+    cu = torch.tensor([0] + lens).cumsum(0)
+    T, n = int(cu[-1]), len(lens)
+    x = ref.inputs(1, T, H, D, dtype=dtype, w=w, seed=34)
+    x["s0"], x["d_s"] = 0.1 * torch.randn(1, H, D, D, generator=g), 0.1 * torch.randn(n, H, D, D, generator=g)
+    want = sequences_alone(x, cu[:-1].tolist(), lens, 1)
+    want["ds0"] = want["ds0"].sum(0, keepdim=True)
+    a = {q: x[q].cuda().requires_grad_(True) for q in ("r", "w", "k", "v", "s0")}
+    d_o, d_s = x["d_o"].cuda(), x["d_s"].cuda()
+    p = ro.PackedSequences(cu, "cuda")
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    o, s = ro.linear_attention_varlen(a["r"], a["w"], a["k"], a["v"], p, initial_state=a["s0"])
+    grads = torch.autograd.grad((o, s), list(a.values()), (d_o, d_s))
+    used = torch.cuda.max_memory_allocated() - before
+    C, state, tokens = 64, H * D * D * 4, T * H * D * (torch.finfo(dtype).bits // 8)
+    # states and their gradients, o, s, the four token gradients and what the engine copies of them, dh0 and its sum, small things
+    assert used <= 2 * (T // C + 2 * n) * state + 3 * n * state + 8 * tokens + (1 << 22), (used, T // C, n, state)
+    got = dict(zip(["o", "s", "dr", "dw", "dk", "dv", "ds0"], [o, s, *grads]))
+    ref.check(got, want, dtype)
