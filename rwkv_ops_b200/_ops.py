@@ -58,6 +58,25 @@ def _register_fakes():
     def kept(r, n):
         return r.new_empty((n,), dtype=torch.uint8)
 
+    # The operators that are called as they are, without a composite one that checks and lays out before them: they refuse what their kernels'
+    # hosts refuse, and what they return is contiguous, whatever the arguments' strides.
+    def need(ok, text):
+        if not ok:
+            raise ValueError(text)
+
+    def step_tokens(r, rest, state):
+        B, H, V, D = state.shape
+        need(r.device.type == "cuda" and state.device == r.device and all(x.device == r.device and x.shape == r.shape for x in rest),
+             "token tensors must agree in shape and device")
+        need(r.dim() in (3, 4) and r.shape[0] == B and r.shape[-2] == H and r.shape[-1] == D == V and (r.dim() == 3 or r.shape[1] == 1),
+             f"expected token tensors [{B}, 1, {H}, {D}] or [{B}, {H}, {D}], got {tuple(r.shape)}")
+        need(state.is_contiguous() and state.dtype in (torch.float32, torch.bfloat16), "expected a contiguous float32 or bfloat16 state")
+
+    def beam_parents(parents, state):
+        need(parents.dim() == 2 and parents.device == state.device and not parents.is_floating_point() and not parents.is_complex()
+             and parents.numel() == state.shape[0] and 1 <= parents.shape[1] <= 32,
+             f"parents must be [groups, beams], at most 32 beams and {state.shape[0]} in all, got {tuple(parents.shape)}")
+
     def dims(r, head_first):
         B, T, H, K = r.shape
         return (B, H, T, K) if head_first else (B, T, H, K)
@@ -76,7 +95,8 @@ def _register_fakes():
 
     @fake("rwkv_ops_b200::rwkv7_decode_step")
     def _(r, w, k, v, a, b, state):
-        return torch.empty_like(r)
+        step_tokens(r, (w, k, v, a, b), state)
+        return r.new_empty(r.shape)
 
     @fake("rwkv_ops_b200::rwkv7_fwd_varlen")
     def _(r, w, k, v, a, b, seq_start, seq_len, max_len, h0, keep):
@@ -132,13 +152,31 @@ def _register_fakes():
 
     @fake("rwkv_ops_b200::linattn_step")
     def _(r, w, k, v, state, parents):
-        return torch.empty_like(r)
+        step_tokens(r, (k, v), state)
+        need(w.device == r.device and (w.dim() == 1 and w.shape[0] == r.shape[-2] or w.shape == r.shape[:-1]),
+             f"w must be [{r.shape[-2]}] or one number per token and head, got {tuple(w.shape)}")
+        need(r.shape[-1] in (64, 128), f"head size must be 64 or 128, got {r.shape[-1]}")
+        if parents is not None:
+            beam_parents(parents, state)
+        return r.new_empty(r.shape)
 
     @fake("rwkv_ops_b200::reorder_states")
     def _(state, parents):
+        need(state.device.type == "cuda" and state.dim() >= 1 and state.is_contiguous() and state.numel() > 0,
+             f"expected a contiguous CUDA tensor of states, got {tuple(state.shape)}")
+        row = state.numel() // state.shape[0] * state.element_size()
+        need(row % 16 == 0, f"a state must be a multiple of 16 bytes, got {row}")
+        beam_parents(parents, state)
         return None
 
     @fake("rwkv_ops_b200::beam_select")
     def _(logits, scores, finished, eos):
-        return (torch.empty_like(scores, dtype=torch.float32), *(torch.empty_like(scores, dtype=torch.int64) for _ in range(2)),
+        need(logits.device.type == "cuda" and logits.dim() == 3 and logits.numel() > 0,
+             f"expected logits [groups, beams, vocabulary], got {tuple(logits.shape)}")
+        need(scores.device == logits.device and scores.shape == logits.shape[:2],
+             f"scores must be {list(logits.shape[:2])}, got {tuple(scores.shape)}")
+        need(logits.shape[1] <= 32 and logits.shape[2] <= 1 << 30, f"at most 32 beams and 2^30 tokens, got {tuple(logits.shape)}")
+        need(eos < logits.shape[2] and (eos >= 0 or finished is None), f"eos must be a token, got {eos}")
+        need(finished is None or (finished.device == logits.device and finished.shape == scores.shape), "finished must be like scores")
+        return (*(scores.new_empty(scores.shape, dtype=t) for t in (torch.float32, torch.int64, torch.int64)),
                 scores.new_empty(scores.shape if eos >= 0 else (0,), dtype=torch.bool))
