@@ -140,7 +140,12 @@ Tensor bytes_if_any(size_t n, const Tensor& like) {
 size_t size_of(const Tensor& x) { return x.defined() ? (size_t)x.numel() : 0; }
 void* stream_of(const Tensor& x) { return c10::cuda::getCurrentCUDAStream(x.device().index()).stream(); }
 
+// Whether a call is to be differentiated.  Forward-mode derivatives are refused: the operators have none, and a call that goes past autograd
+// because no input requires a gradient would drop the tangents.
 bool any_requires_grad(at::ArrayRef<const Tensor*> xs, const OptTensor& s) {
+  const auto tangent = [](const Tensor& x) { return x.defined() && x._fw_grad(/*level=*/0).defined(); };
+  for (const Tensor* x : xs) TORCH_CHECK_NOT_IMPLEMENTED(!tangent(*x), "rwkv_ops_b200: forward-mode derivatives are not implemented");
+  TORCH_CHECK_NOT_IMPLEMENTED(!has(s) || !tangent(*s), "rwkv_ops_b200: forward-mode derivatives are not implemented");
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* x : xs)
     if (x->requires_grad()) return true;

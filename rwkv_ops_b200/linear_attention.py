@@ -99,6 +99,7 @@ class LinearAttentionDecodeState:
     Beam search: the sequences are ``groups * beams``, the beams of a search next to each other.  With ``parents`` (``[groups, beams]``, what
     ``beam_select`` returns) beam ``j`` of a search goes on from the state that beam ``parents[j]`` of that search had: the step reads it from there, so the
     reordering costs nothing.  ``reorder`` does it alone.  At most 32 beams; entries outside the search are clamped.
+    Steps are not differentiated.
     """
 
     def __init__(self, batch: int, heads: int, *, head_size: int = 64, state_dtype: torch.dtype = torch.float32, device="cuda",
