@@ -191,6 +191,11 @@ void check_state(const OptTensor& s, const Tensor& r, const SymInt& B, const Sym
                     "initial_state must be [", B, " or 1, ", H, ", ", N, ", ", N, "], got ", s->sym_sizes());
 }
 
+// a state that steps work on in place: the kernels take its last two sizes from the tokens
+void check_resident(const Tensor& state) {
+  TORCH_CHECK_VALUE(state.dim() == 4 && state.size(2) == state.size(3), "expected states [batch, heads, head size, head size], got ", state.sizes());
+}
+
 // ---------------------------------------------------------------------------------------------
 // RWKV7, dense
 // ---------------------------------------------------------------------------------------------
@@ -345,6 +350,8 @@ std::tuple<Tensor, Tensor> generalized_delta_rule(const Tensor& r, const Tensor&
 Tensor rwkv7_decode_step(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, const Tensor& a,
                          const Tensor& b, Tensor state) {
   check_tokens(r, {&w, &k, &v, &a, &b}, (int)r.dim());
+  check_resident(state);
+  TORCH_CHECK_VALUE(state.size(3) == HEAD, "expected states of head size 64, got ", state.sizes());
   const int64_t B = state.size(0), H = state.size(1);
   TORCH_CHECK_VALUE((r.dim() == 3 || (r.dim() == 4 && r.size(1) == 1)) && r.size(0) == B && r.size(r.dim() - 2) == H &&
                         r.size(-1) == HEAD && state.is_contiguous() && state.device() == r.device(),
@@ -902,6 +909,7 @@ void changed(const Tensor& state) {
 
 Tensor linattn_step(const Tensor& r, const Tensor& w, const Tensor& k, const Tensor& v, Tensor state, const OptTensor& parents) {
   check_tokens(r, {&k, &v}, (int)r.dim());
+  check_resident(state);
   const int64_t B = state.size(0), H = state.size(1), D = state.size(3);
   TORCH_CHECK_VALUE((r.dim() == 3 || (r.dim() == 4 && r.size(1) == 1)) && r.size(0) == B && r.size(r.dim() - 2) == H &&
                         r.size(-1) == D && state.is_contiguous() && state.device() == r.device(),
