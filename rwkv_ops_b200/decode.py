@@ -37,7 +37,8 @@ class Rwkv7DecodeState:
             if initial_state.dim() != 4 or tuple(initial_state.shape[1:]) != shape[1:] \
                     or initial_state.shape[0] not in (1, batch):
                 raise ValueError(f"initial_state must be [{batch} or 1, {heads}, 64, 64], got {tuple(initial_state.shape)}")
-            self.state = initial_state.expand(shape).to(state_dtype).contiguous().clone()
+            self.state = torch.empty(shape, dtype=state_dtype, device=initial_state.device)
+            self.state.copy_(initial_state.detach())      # (one state may serve all sequences)
         else:
             self.state = torch.zeros(shape, dtype=state_dtype, device=device)
         if not self.state.is_cuda:

@@ -112,7 +112,8 @@ class LinearAttentionDecodeState:
         if initial_state is not None:
             _lib.require_cuda(initial_state)
             _check_state(initial_state, batch, heads, head_size)
-            self.state = initial_state.detach().expand(shape).to(state_dtype).contiguous().clone()
+            self.state = torch.empty(shape, dtype=state_dtype, device=initial_state.device)
+            self.state.copy_(initial_state.detach())      # (one state may serve all sequences)
         else:
             self.state = torch.zeros(shape, dtype=state_dtype, device=device)
         if not self.state.is_cuda:
