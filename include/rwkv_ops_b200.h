@@ -372,7 +372,7 @@ int rwkvb200_reorder_states(void* state, const int64_t* parents, int groups, int
 /* ------------------------------------------------------------------------------------------
  * Beam search (no counterpart in the reference): the best continuations of `groups` searches of `beams` (at most 32) beams over
  * `vocab` tokens.  Candidate (i, t) of a group has the score scores[i] + logits[i][t] - log sum_u exp(logits[i][u]); the `beams` best are
- * returned in descending order, ties to the lowest i * vocab + t.  A beam marked in `finished` (may be NULL) goes on with eos alone,
+ * returned in descending order (float64), ties to the lowest i, then to the larger logit, then to the lowest t.  A beam marked in `finished` (may be NULL) goes on with eos alone,
  * at the score it has.  finished_out (may be NULL): whether the parent had finished or the token is eos.  eos < 0: none.
  * logits: last dimension contiguous, strides in elements; NaN and +inf count as -inf.
  * ---------------------------------------------------------------------------------------- */

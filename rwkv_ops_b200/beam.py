@@ -24,7 +24,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
 
     ``logits``: ``[groups, beams, vocabulary]`` (float32, bfloat16 or float16, last dimension contiguous, any other strides); ``scores``:
     ``[groups, beams]``, the beams' summed log-probabilities (``-inf`` for a beam that does not exist yet).  Candidate ``(i, t)`` has the score
-    ``scores[i] + log_softmax(logits[i])[t]``; candidates are compared in float64, equal ones go to the lower beam, then to the lower token.
+    ``scores[i] + log_softmax(logits[i])[t]``; candidates are compared in float64, equal ones go to the lower beam, then to the larger logit, then to the lower token.
     ``finished`` (bool, like ``scores``; needs ``eos``): such a beam goes on with ``eos`` alone, at the score it has.
 
     Returns ``(scores, parents, tokens)``, each ``[groups, beams]`` in descending order of scores (float32, int64, int64), and with ``eos``

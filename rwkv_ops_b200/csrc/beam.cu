@@ -1,7 +1,7 @@
 // Beam search: the W best continuations of W beams over the vocabulary, in one launch and one pass over the logits.
 //
 // Per group of W beams with running scores s_i (log-probabilities) and logits x_i[V]:
-//   candidate (i, t) has the score s_i + x_i[t] - log sum_u e^{x_i[u]};   the W best, ties to the lowest i V + t.
+//   candidate (i, t) has the score s_i + x_i[t] - log sum_u e^{x_i[u]};   the W best, ties to the lowest i, then to the larger logit, then to the lowest t.
 //
 // What bounds it is reading the logits once.  The W best of a row come from its own logits in their own order.  A warp streams a slice of a row and
 // keeps, for each lane, the running maximum, the tile it is in, the largest of the other tiles and the running sum: some 250 instructions for 512 tokens, where
@@ -36,12 +36,12 @@ constexpr float LN2 = 0.6931471805599453f, LOG2E_LO = (float)(1.4426950408889634
 // A list of the best (value, index) of a warp, sorted, entry l in lane l; entries beyond the first `n` lanes do not matter.
 template <typename F, typename I>
 struct Best {
-  static constexpr I NONE = sizeof(I) == 8 ? (I)LLONG_MAX : (I)INT_MAX;
+  static constexpr I NONE = (I)INT_MAX;
   F v = (F)NEG;
   I i = NONE;
 };
 typedef Best<float, int> RowBest;              // of a row: its tokens
-typedef Best<double, long long> GroupBest;     // of a group: i V + t
+constexpr int NO_ORDER = INT_MAX;              // of a group's candidates
 template <typename F, typename I>
 __device__ __forceinline__ bool before(F v, I i, F v2, I i2) { return v > v2 || (v == v2 && i < i2); }
 // (x, j), the same in every lane, into the list
@@ -164,7 +164,7 @@ __device__ __forceinline__ int key_token(Key k) { return (int)~(uint32_t)k; }
 struct Smem {
   union {
     Key key[MAXC * NWARP * MAXW];                  // in the first CTA: of every warp of the cluster, the W best of its slice [warp][W]
-    struct { double score[MAXW * MAXW + MAXW]; long long at[MAXW * MAXW + MAXW]; } last;      // then the group's candidates
+    struct { double score[MAXW * MAXW + MAXW]; int order[MAXW * MAXW + MAXW], token[MAXW * MAXW + MAXW]; } last;      // then the group's candidates
   };
   Key best[MAXW][MAXW];                            // of a row: its W best
   double s[MAXC * NWARP];                          // of every warp of the cluster: the sum relative to its maximum
@@ -340,7 +340,8 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
     if (place < W) sm.best[e / n_key][place] = mine;
   }
   __syncthreads();
-  // The group's candidates: the rows' W best and, behind them, the finished beams' eos.
+  // The group's candidates: the rows' W best and, behind them, the finished beams' eos.  Of equal scores the lower beam's comes first, and of one beam's the one
+  // that its own order puts first: by logits, which may differ where the sums do not, then by tokens (for impossible candidates and a finished beam by tokens).
   const int n_last = W * W + W;
   for (int e = threadIdx.x; e < n_last; e += NWARP * 32) {
     const int i = e < W * W ? e / W : e - W * W, at = e - i * W;
@@ -362,18 +363,21 @@ beam_select_kernel(const T* __restrict__ logits, long long stride_g, long long s
       if (key_logit(k) != NEG) score = sm.shift[i] + ((double)key_logit(k) - sm.top[i]);
     }
     sm.last.score[e] = score;
-    sm.last.at[e] = t < 0 || t >= V ? GroupBest::NONE : (long long)i * V + t;
+    sm.last.token[e] = t;
+    // (a finished beam's tokens: eos before the W-th or behind all of the others)
+    const int place = e < W * W ? over && at >= (int)eos ? at + 1 : at : (int)(eos < W ? eos : W);
+    sm.last.order[e] = t < 0 || t >= V ? NO_ORDER : i * (W + 1) + place;
   }
   __syncthreads();
   for (int e = threadIdx.x; e < n_last; e += NWARP * 32) {
     const double score = sm.last.score[e];
-    const long long j = sm.last.at[e];
-    if (j == GroupBest::NONE) continue;
+    const int j = sm.last.order[e];
+    if (j == NO_ORDER) continue;
     int place = 0;
 #pragma unroll 4
-    for (int q = 0; q < n_last; ++q) place += before(sm.last.score[q], sm.last.at[q], score, j);
+    for (int q = 0; q < n_last; ++q) place += before(sm.last.score[q], sm.last.order[q], score, j);
     if (place < W) {
-      const long long at = (long long)g * W + place, parent = j / V, t = j - parent * V;
+      const long long at = (long long)g * W + place, parent = e < W * W ? e / W : e - W * W, t = sm.last.token[e];
       scores_out[at] = (float)score;
       parents[at] = parent;
       tokens[at] = t;
