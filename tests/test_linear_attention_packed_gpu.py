@@ -117,3 +117,39 @@ def test_one_long_sequence_among_many_short_ones(dtype, D, w, n_short, keep, mon
     assert used <= 2 * (T // C + 2 * n) * state + 3 * n * state + 8 * tokens + (1 << 22), (used, T // C, n, state)
     got = dict(zip(["o", "s", "dr", "dw", "dk", "dv", "ds0"], [o, s, *grads]))
     ref.check(got, want, dtype)
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 256, 257, 513])
+def test_as_many_sequences_as_are_put_in_order_and_more(n):
+    """The order in which sequences are worked on is not seen: together they are what two halves of them are, and each is its definition."""
+    import rwkv_ops_b200 as ro
+    g = torch.Generator(device="cuda").manual_seed(n)
+    H = 2
+    lens = torch.randint(1, 300, (n,), generator=g, device="cuda").cpu()
+    cu = torch.cat([torch.zeros(1, dtype=torch.long), lens.cumsum(0)])
+    T = int(cu[-1])
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")
+    x = [rand(1, T, H, 64).to(BF16), -3 + rand(1, T, H), rand(1, T, H, 64).to(BF16) / 8, rand(1, T, H, 64).to(BF16)]
+    d_o, d_s = rand(1, T, H, 64).to(BF16), 0.1 * rand(n, H, 64, 64)
+
+    def call(a, b):      # sequences a .. b - 1
+        cut = slice(int(cu[a]), int(cu[b]))
+        y = [t[:, cut].contiguous().requires_grad_(True) for t in x]
+        o, s = ro.linear_attention_varlen(*y, cu[a:b + 1] - cu[a])
+        return [o, *torch.autograd.grad((o, s), y, (d_o[:, cut].contiguous(), d_s[a:b].contiguous()))], s
+
+    tokens, states = call(0, n)
+    k = n // 2
+    parts = [call(0, k), call(k, n)]
+    # (the halves may be cut into other stretches, whose starts are summed in another order: float32's last bits)
+    for i, t in enumerate(tokens):
+        want = torch.cat([p[0][i] for p in parts], 1)
+        tol = ref.tolerance("dw" if i == 2 else "o", BF16)
+        assert float((t.double() - want.double()).norm() / want.double().norm()) <= tol
+    assert float((states - torch.cat([p[1] for p in parts])).norm() / states.norm()) <= ref.tolerance("s", F32)
+    for i in range(0, n, max(1, n // 7)):      # and single ones against the definition
+        cut = slice(int(cu[i]), int(cu[i + 1]))
+        y = {q: t[:, cut].cpu() for q, t in zip("rwkv", x)}
+        y.update(s0=None, d_o=d_o[:, cut].cpu(), d_s=d_s[i:i + 1].cpu())
+        got = dict(zip(["o", "dr", "dw", "dk", "dv"], [t[:, cut] for t in tokens]))
+        ref.check({**got, "s": states[i:i + 1]}, ref.with_gradients(y), BF16)
