@@ -153,3 +153,31 @@ def test_as_many_sequences_as_are_put_in_order_and_more(n):
         y.update(s0=None, d_o=d_o[:, cut].cpu(), d_s=d_s[i:i + 1].cpu())
         got = dict(zip(["o", "dr", "dw", "dk", "dv"], [t[:, cut] for t in tokens]))
         ref.check({**got, "s": states[i:i + 1]}, ref.with_gradients(y), BF16)
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F32, 64), (F16, 128)])
+@pytest.mark.parametrize("name", ["r", "w", "k", "v", "d_o", "d_s", "s0"])
+def test_a_sequence_leaves_its_neighbours_alone(name, dtype, D):
+    """NaN in any argument of one sequence, which begins and ends inside its neighbours' chunks, changes no bit of theirs."""
+    import rwkv_ops_b200 as ro
+    cu, H = [0, 70, 131, 195, 452], 2
+    x = ref.inputs(1, cu[-1], H, D, dtype=dtype, seed=35)
+    g = torch.Generator().manual_seed(36)
+    x["s0"], x["d_s"] = 0.1 * torch.randn(4, H, D, D, generator=g), 0.1 * torch.randn(4, H, D, D, generator=g)
+
+    def call(x):
+        a = {q: x[q].cuda().requires_grad_(True) for q in ("r", "w", "k", "v", "s0")}
+        o, s = ro.linear_attention_varlen(a["r"], a["w"], a["k"], a["v"], cu, initial_state=a["s0"])
+        return [o, s, *torch.autograd.grad((o, s), list(a.values()), (x["d_o"].cuda(), x["d_s"].cuda()))]
+
+    bad = dict(x)
+    bad[name] = x[name].clone()
+    if name in ("s0", "d_s"):
+        bad[name][2] = float("nan")
+    else:
+        bad[name][:, 131:195] = float("nan")
+    for p, q in zip(call(x), call(bad)):
+        if p.shape[0] == 4:
+            assert torch.equal(p[[0, 1, 3]], q[[0, 1, 3]])
+        else:
+            assert torch.equal(p[:, :131], q[:, :131]) and torch.equal(p[:, 195:], q[:, 195:])
