@@ -5,7 +5,9 @@
 // Precision.  r, k, v, d_o are bfloat16 and enter products as they are.  The keys (queries) that are added to the state (its gradient) carry a decay and are split
 // into three bfloat16 parts (three products, exact to float32's last bits: states go from chunk to chunk and are float32).  The states that meet v, k and d_o in the
 // backward are hi + lo (two products, 2^-17): from them come gradients of tokens, and of dw the part that reaches beyond its chunk; room for a third
-// part is not there.  A and E are rounded once to bfloat16, as is the state that meets r in the forward: those results are rounded to bfloat16 anyway.
+// part is not there.  The smallest part goes first: an accumulator in TMEM cuts off what a product adds below its own last bit, and 24 steps of a chunk at
+// full size leave states 5e-7 too small, 8 of them 1.3e-7.  A and E are rounded once to bfloat16, as is the state that meets r in the forward: those results are
+// rounded to bfloat16 anyway.
 //
 // Work is cut into items, a stretch of consecutive chunks of one (sequence, head).  With as many units as the device holds CTAs, an item is a unit.  With
 // fewer, a unit is several parts: a first kernel finds what each adds to the state, keys and values only, and then all parts are walked at once from the state

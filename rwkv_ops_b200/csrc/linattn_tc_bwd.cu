@@ -257,12 +257,12 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
         umma_tile<128, 128, 0, 0>(tmem_addr(tm, 0, TM_S), smem_u32(sm.r), smem_u32(sm.k), false);
         umma_tile<128, 128, 0, 0>(tmem_addr(tm, 0, TM_P), smem_u32(sm.d_o), smem_u32(sm.v), false);
         umma_commit(&sm.bar_1);
-        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XR), smem_u32(sm.d_o), smem_u32(sm.S[0]), false);
-        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XR), smem_u32(sm.d_o), smem_u32(sm.S[1]), true);
-        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XK), smem_u32(sm.v), smem_u32(sm.dS[0]), false);
-        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XK), smem_u32(sm.v), smem_u32(sm.dS[1]), true);
-        umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_XV), smem_u32(sm.k), smem_u32(sm.dS[0]), false);
-        umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_XV), smem_u32(sm.k), smem_u32(sm.dS[1]), true);
+        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XR), smem_u32(sm.d_o), smem_u32(sm.S[1]), false);
+        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XR), smem_u32(sm.d_o), smem_u32(sm.S[0]), true);
+        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XK), smem_u32(sm.v), smem_u32(sm.dS[1]), false);
+        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XK), smem_u32(sm.v), smem_u32(sm.dS[0]), true);
+        umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_XV), smem_u32(sm.k), smem_u32(sm.dS[1]), false);
+        umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_XV), smem_u32(sm.k), smem_u32(sm.dS[0]), true);
         umma_commit(&sm.bar_x);
       }
       if (warp == STORE && elect_one()) {
@@ -408,9 +408,9 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
         ok = mbar_wait(&sm.bar_r, ph, status, 515) && ok;
         tc_fence_after();
         if (elect_one()) {
-          umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.rhi), false);
+          umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.v), false);
           umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.rlo), true);
-          umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.v), true);
+          umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_W), smem_u32(sm.d_o), smem_u32(sm.rhi), true);
           umma_commit(&sm.bar_2);
         }
       }

@@ -225,9 +225,9 @@ la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int 
           umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_O2), smem_u32(sm.A[0]), smem_u32(sm.v), false);
           umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_O2), smem_u32(sm.A[1]), smem_u32(sm.v) + TILE_BYTES, true);
         }
-        umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.k), false);
+        umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.r), false);
         umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.klo), true);
-        umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.r), true);
+        umma_tile<64, 64, 1, 1, 8>(tmem_addr(tm, 0, TM_U), smem_u32(sm.v), smem_u32(sm.k), true);
         umma_commit(&sm.bar_2);
       }
       ok = mbar_wait(&sm.bar_2, ph, status, 503) && ok;

@@ -136,7 +136,7 @@ def test_as_many_sequences_as_are_put_in_order_and_more(n):
         cut = slice(int(cu[a]), int(cu[b]))
         y = [t[:, cut].contiguous().requires_grad_(True) for t in x]
         o, s = ro.linear_attention_varlen(*y, cu[a:b + 1] - cu[a])
-        return [o, *torch.autograd.grad((o, s), y, (d_o[:, cut].contiguous(), d_s[a:b].contiguous()))], s
+        return [o.detach(), *torch.autograd.grad((o, s), y, (d_o[:, cut].contiguous(), d_s[a:b].contiguous()))], s.detach()
 
     tokens, states = call(0, n)
     k = n // 2
