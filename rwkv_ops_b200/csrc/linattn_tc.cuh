@@ -3,9 +3,9 @@
 // token's row.
 //
 // Precision.  r, k, v, d_o are bfloat16 and enter products as they are.  The keys (queries) that are added to the state (its gradient) carry a decay and are split
-// into three bfloat16 parts (three products, exact to float32's last bits: states go from chunk to chunk and are float32).  The states that meet v, k and d_o in the
-// backward are hi + lo (two products, 2^-17): from them come gradients of tokens, and of dw the part that reaches beyond its chunk; room for a third
-// part is not there.  The smallest part goes first: an accumulator in TMEM cuts off what a product adds below its own last bit, and 24 steps of a chunk at
+// into three bfloat16 parts (three products, exact to float32's last bits: states go from chunk to chunk and are float32).  The states that meet v and d_o in the
+// backward are in three parts, too, as from these products comes the part of dw that reaches beyond its chunk (with two, 2^-17 of an element, dw was
+// off by 1.2e-6 instead of 3e-7); the one that meets k, for dv alone, is in two.  The smallest part goes first: an accumulator in TMEM cuts off what a product adds below its own last bit, and 24 steps of a chunk at
 // full size leave states 5e-7 too small, 8 of them 1.3e-7.  A and E are rounded once to bfloat16, as is the state that meets r in the forward: those results are
 // rounded to bfloat16 anyway.
 //

@@ -13,7 +13,7 @@ struct BwdSmem {
   unsigned char r[TOK_BYTES], k[TOK_BYTES], v[TOK_BYTES], d_o[TOK_BYTES];
   unsigned char rhi[TOK_BYTES], rlo[TOK_BYTES];      // e^{L_i} r_i, of which the third part takes the place of v; dr and dk are staged here afterwards
   unsigned char A[2][TOK_BYTES], E[2][TOK_BYTES];    // [token i][token j], two times 64 columns; dv is staged in the halves that are zero, see stage_v
-  unsigned char S[2][TILE_BYTES], dS[2][TILE_BYTES]; // the state before the chunk and the gradient of the one after it, hi and lo, [v][k]
+  unsigned char S[3][TILE_BYTES], dS[2][TILE_BYTES]; // the state before the chunk and the gradient of the one after it in three parts, [v][k] (the last: see dS3)
   Decays dec[2];
   float g[3][CT], decay[3];      // g and e^{Lc} of this chunk, the next one (being made) and the one before (whose dw is)
   double dw_sum[32];
@@ -45,34 +45,38 @@ __device__ __forceinline__ float column_sum(float (&x)[16], int lane) {
   }
   return x[0] + __shfl_xor_sync(0xffffffffu, x[0], 16);
 }
-// 16 values of a row, columns col0 .. (a multiple of 8), as hi and lo tiles
-__device__ __forceinline__ void store_split16(unsigned char* hi_t, unsigned char* lo_t, int row, int col0, const float* x) {
+// 16 values of a row, columns col0 .. (a multiple of 8), as the tiles of their three bfloat16 parts
+__device__ __forceinline__ void store_split16(unsigned char (*hi_lo)[TILE_BYTES], unsigned char* third, int row, int col0, const float* x) {
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    uint32_t h[4], l[4];
+    uint32_t h[4], l[4], m[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float a = x[8 * c + 2 * e], b = x[8 * c + 2 * e + 1];
+      float a = x[8 * c + 2 * e], b = x[8 * c + 2 * e + 1];
       h[e] = pack_bf16(a, b);
-      l[e] = pack_bf16(a - bf16_lo(h[e]), b - bf16_hi(h[e]));
+      a -= bf16_lo(h[e]); b -= bf16_hi(h[e]);
+      l[e] = pack_bf16(a, b);
+      m[e] = pack_bf16(a - bf16_lo(l[e]), b - bf16_hi(l[e]));
     }
     const uint32_t off = tile_chunk_off(row, (col0 >> 3) + c);
-    *reinterpret_cast<uint4*>(hi_t + off) = make_uint4(h[0], h[1], h[2], h[3]);
-    *reinterpret_cast<uint4*>(lo_t + off) = make_uint4(l[0], l[1], l[2], l[3]);
+    *reinterpret_cast<uint4*>(hi_lo[0] + off) = make_uint4(h[0], h[1], h[2], h[3]);
+    *reinterpret_cast<uint4*>(hi_lo[1] + off) = make_uint4(l[0], l[1], l[2], l[3]);
+    *reinterpret_cast<uint4*>(third + off) = make_uint4(m[0], m[1], m[2], m[3]);
   }
 }
 
 // One item: the chunks of a stretch from the last to the first, the gradient of the state in registers.  Per chunk two batches of products:
-//   r k^T, d_o v^T; d_o S, v dS, k dS^T     the first two are waited for, the others run on while A and E are made of them
+//   r k^T, d_o v^T; d_o S, v dS, k dS^T     the first two are waited for, the others run on while A and E are made of them (all but where the third part of dS is)
 //   E k, E^T r, A^T d_o; d_o^T (scaled r)   after A and E have been stored; meanwhile the states' part of dw
 // then the three gradients are put together and staged, and leave while the next chunk is worked on.
-// Sixteen warps, one CTA to an SM (all of TMEM, 222 KB): warp w reads token rows 32 (w % 4) .. and a quarter of the columns; the six warps whose block of pairs lies
+// Sixteen warps, one CTA to an SM (all of TMEM, 226 KB): warp w reads token rows 32 (w % 4) .. and a quarter of the columns; the six warps whose block of pairs lies
 // above the diagonal clear it and do the single-thread jobs, the next chunk's decays and the dw of the chunk before.  Within a chunk warps wait for products
 // and rows only, and the issuing threads for the warps; all warps meet once, at its end.
 //
-// What bounds it: shared memory.  Operands split into hi and lo, scores, factors and staged gradients are some 767 KB of it a chunk, 6k cycles at 128 bytes each,
-// of the 10k cycles (5.4 us) that a chunk takes; the rest are waits between the batches (tensor pipe 22 % of the cycles, issue slots 41 %).  Measured: B 8 x T 4096,
-// H 32, 361 us for 1.07 GB (3 TB/s); 256 items on 148 SMs are two waves.
+// What bounds it: the chain of a chunk's steps, products, TMEM reads, rounding and storing, products, with one CTA to wait in.  No unit is near its limit (tensor pipe
+// 22 % of the cycles, issue slots 41 %; shared memory moves some 800 KB a chunk, 6k of 11k cycles at 128 bytes each), and leaving out the
+// column sums, the stores of A and E, or the copies of the gradients changes a chunk by less than 6 %.  Measured: B 8 x T 4096, H 32, 390 us for 1.07 GB
+// (2.7 TB/s; 365 with the states in two parts: products 10, splitting and storing 6 in a chunk's last step, waiting 9); 256 items on 148 SMs are two waves.
 template <bool PACKED>
 __global__ void __launch_bounds__(NTHR, 1)
 la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, const float* __restrict__ states, bf16* __restrict__ dr,
@@ -159,11 +163,14 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       S0[4 * j] = f.x; S0[4 * j + 1] = f.y; S0[4 * j + 2] = f.z; S0[4 * j + 3] = f.w;
     }
   };
+  // The third part of the gradient lies where the last rows' left half of E comes later: that of the chunk before has been read, that of this one is stored after the
+  // products with the states.
+  unsigned char* dS3 = sm.E[0] + TILE_BYTES;
   // the gradient of a chunk's state into its tiles, and its product with the state
   auto put_tiles = [&](int ph) {
     float s = 0.f;
     if (st_lane) {
-      store_split16(sm.dS[0], sm.dS[1], srow, 16 * qt, dS);
+      store_split16(sm.dS, dS3, srow, 16 * qt, dS);
 #pragma unroll
       for (int j = 0; j < 16; ++j) s = fmaf(S0[j], dS[j], s);
     }
@@ -232,7 +239,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       if (lane == 0) sm.decay[0] = sm.dec[0].all;
     }
     get_kept(x.hi - 1);
-    if (st_lane) store_split16(sm.S[0], sm.S[1], srow, 16 * qt, S0);
+    if (st_lane) store_split16(sm.S, sm.S[2], srow, 16 * qt, S0);
     put_tiles(0);
     fence_async_smem();
     __syncthreads();
@@ -257,13 +264,15 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
         umma_tile<128, 128, 0, 0>(tmem_addr(tm, 0, TM_S), smem_u32(sm.r), smem_u32(sm.k), false);
         umma_tile<128, 128, 0, 0>(tmem_addr(tm, 0, TM_P), smem_u32(sm.d_o), smem_u32(sm.v), false);
         umma_commit(&sm.bar_1);
-        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XR), smem_u32(sm.d_o), smem_u32(sm.S[1]), false);
+        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XR), smem_u32(sm.d_o), smem_u32(sm.S[2]), false);
+        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XR), smem_u32(sm.d_o), smem_u32(sm.S[1]), true);
         umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XR), smem_u32(sm.d_o), smem_u32(sm.S[0]), true);
-        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XK), smem_u32(sm.v), smem_u32(sm.dS[1]), false);
+        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XK), smem_u32(sm.v), smem_u32(dS3), false);
+        umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XK), smem_u32(sm.v), smem_u32(sm.dS[1]), true);
         umma_tile<128, 64, 0, 1>(tmem_addr(tm, 0, TM_XK), smem_u32(sm.v), smem_u32(sm.dS[0]), true);
-        umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_XV), smem_u32(sm.k), smem_u32(sm.dS[1]), false);
-        umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_XV), smem_u32(sm.k), smem_u32(sm.dS[0]), true);
         umma_commit(&sm.bar_x);
+        umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_XV), smem_u32(sm.k), smem_u32(sm.dS[1]), false);      // (bar_2 waits for these, too)
+        umma_tile<128, 64, 0, 0>(tmem_addr(tm, 0, TM_XV), smem_u32(sm.k), smem_u32(sm.dS[0]), true);
       }
       if (warp == STORE && elect_one()) {
         if (i) {
@@ -277,6 +286,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       tc_fence_after();
       unsigned char* At = sm.A[qt >> 1] + (row >> 6) * TILE_BYTES;
       unsigned char* Et = sm.E[qt >> 1] + (row >> 6) * TILE_BYTES;
+      if (wq >= 2 && qt < 2) ok = mbar_wait(&sm.bar_x, ph, status, 514) && ok;      // (the third part has been read)
       if (qt <= wq) {
         const bool diag = qt == wq;
         float run = 0.f, cs[2];      // of the pairs' part of dg: the sum of a row so far, and of its columns
@@ -355,7 +365,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       }
       tc_fence_before();
       arrive(sm.bar_ae);
-      // the scaled r in three parts, 8 tokens to a warp (B 8 x T 4096, H 32: 361 us; by the three warps that have the least else to do 385; in two parts 357)
+      // the scaled r in three parts, 8 tokens to a warp (B 8 x T 4096, H 32, with states in two parts: 361 us; by the three warps that have the least else to do 385)
       ok = mbar_wait(&sm.bar_free, ph, status, 518) && ok;
       ok = mbar_wait(&sm.bar_x, ph, status, 514) && ok;
       tc_fence_after();
@@ -402,7 +412,7 @@ la_tc_bwd_kernel(const float* __restrict__ w, const float* __restrict__ d_ht, co
       };
       state_part(TM_XR, d.start[row], sm.r, sm.t1[ph][qt]);
       state_part(TM_XK, d.end[row], sm.k, sm.t2[ph][qt]);
-      if (c > x.lo && st_lane) store_split16(sm.S[0], sm.S[1], srow, 16 * qt, S0);      // (the products with this chunk's are done)
+      if (c > x.lo && st_lane) store_split16(sm.S, sm.S[2], srow, 16 * qt, S0);      // (the products with this chunk's are done)
       arrive(sm.bar_read);
       if (warp == ISSUE_W) {
         ok = mbar_wait(&sm.bar_r, ph, status, 515) && ok;

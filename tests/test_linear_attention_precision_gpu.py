@@ -143,3 +143,33 @@ def test_sums_of_one_sign(backward):
     name = "ds0" if backward else "s"
     got, want = run(x)[name].double().cpu(), ref.with_gradients(x)[name]
     assert ((got - want).abs() <= 2.0 ** -20 * want).all(), float(((got - want) / want).abs().max())
+
+
+@pytest.mark.parametrize("side", ["first", "last"])
+def test_gradients_of_decays_that_come_from_one_element(side):
+    """One token reads one element of the first state (adds to one that a gradient of the last state meets): every decay between the two has a gradient of
+    g D S[v][k], D the decay of all of them, and nothing is added up.  Three parts of the state are exact to 2^-24; two exponentials of 2^-22 and some six
+    roundings of 2^-24 make less than 2^-20.  (Two parts leave up to 2^-17.)"""
+    import rwkv_ops_b200 as ro
+    B, T, H = 96, 128, 2
+    x = ref.inputs(B, T, H, dtype=BF16, seed=48, w_mean=-7.0, w_std=0.3, n_state=B)
+    gen = torch.Generator().manual_seed(49)
+    at, vi, ki = torch.arange(B) * 4 // 3, torch.randint(0, 64, (B,), generator=gen), torch.randint(0, 64, (B,), generator=gen)
+    n = torch.arange(B)
+    key, value = torch.zeros(B, T, H, 64, dtype=BF16), torch.zeros(B, T, H, 64, dtype=BF16)
+    key[n, at, :, ki], value[n, at, :, vi] = 1.0, 1.0
+    zero, nothing = torch.zeros(B, T, H, 64, dtype=BF16), torch.zeros(B, H, 64, 64)
+    g = -torch.exp(x["w"].double())
+    t = torch.arange(T)[None]
+    if side == "first":      # r, d_o and the first state
+        r, k, v, d_o, s0, d_s, state = key, zero, zero, value, x["s0"], nothing, x["s0"]
+        D, has = torch.exp(g.cumsum(1))[n, at], t <= at[:, None]
+    else:
+        r, k, v, d_o, s0, d_s, state = zero, key, value, zero, nothing, x["d_s"], x["d_s"]
+        D, has = torch.exp(g.flip(1).cumsum(1).flip(1) - g)[n, at], t > at[:, None]
+    w = x["w"].cuda().requires_grad_(True)
+    o, s = ro.linear_attention(r.cuda(), w, k.cuda(), v.cuda(), initial_state=s0.cuda())
+    got, = torch.autograd.grad((o, s), w, (d_o.cuda(), d_s.cuda()))
+    want = torch.where(has[..., None], g * (D * state.double()[n, :, vi, ki])[:, None], 0)
+    off = (got.double().cpu() - want).abs()
+    assert (off <= 2.0 ** -20 * want.abs()).all(), float((off / want.abs().clamp(min=1e-30)).max())
