@@ -7,7 +7,7 @@
 //
 // What bounds it: float32 multiply-adds at the latency of shared memory that feeds them (issue slots 46 - 54 % used, the multiply-add pipe 33 - 40 %, no other
 // unit above 55 %).  B2 T1024 H16 of 64 in float32, forward and backward, 512 chunks: adding 19 us and scanning 7.5 us in either direction, outputs 37 us,
-// gradients 108 us in 3.5 waves of blocks; the bytes of the tensors alone would take 11.
+// gradients 109 us in 3.5 waves of blocks; the bytes of the tensors alone would take 11.
 #include "linattn.cuh"
 
 namespace rwkvb200 {

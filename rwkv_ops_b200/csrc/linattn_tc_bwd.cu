@@ -74,7 +74,7 @@ __device__ __forceinline__ void store_split16(unsigned char (*hi_lo)[TILE_BYTES]
 // and rows only, and the issuing threads for the warps; all warps meet once, at its end.
 //
 // What bounds it: the chain of a chunk's steps, products, TMEM reads, rounding and storing, products, with one CTA to wait in.  No unit is near its limit (tensor pipe
-// 22 % of the cycles, issue slots 41 %; shared memory moves some 800 KB a chunk, 6k of 11k cycles at 128 bytes each), and leaving out the
+// 27 % of the cycles, issue slots 43 %; shared memory moves some 800 KB a chunk, 6k of 11k cycles at 128 bytes each), and leaving out the
 // column sums, the stores of A and E, or the copies of the gradients changes a chunk by less than 6 %.  Measured: B 8 x T 4096, H 32, 390 us for 1.07 GB
 // (2.7 TB/s; 365 with the states in two parts: products 10, splitting and storing 6 in a chunk's last step, waiting 9); 256 items on 148 SMs are two waves.
 template <bool PACKED>

@@ -39,9 +39,9 @@ constexpr uint32_t TM_S = 0, TM_O2 = 0, TM_O1 = 128;
 // gradient of the state, from the last chunk to the first, with r for keys and d_o for values.
 // Two CTAs share an SM (113 KB each, 256 TMEM columns each), so that one's products and loads run under the other's arithmetic.
 //
-// What bounds it: the steps of a chunk in turn, products, TMEM reads, the threads' rounding and storing, 3.7 us with two CTAs to an SM (tensor pipe 19 % of the
-// cycles, issue slots 28 %); memory a third below a copy's rate.  Measured, H 32: training of B 8 x T 4096, states kept, 160 us for 671 MB (4.2 TB/s); inference of
-// B 4 x T 16384 384 us, 96 of them in the pass over keys and values, for 1086 MB without that pass.
+// What bounds it: the steps of a chunk in turn, products, TMEM reads, the threads' rounding and storing, 4.5 us with two CTAs to an SM, 5 with states kept (tensor pipe 22 % of the
+// cycles, issue slots 30 %); memory a third below a copy's rate.  Measured, H 32: training of B 8 x T 4096, states kept, 160 us for 671 MB (4.2 TB/s); inference of
+// B 4 x T 16384 386 us, 95 of them in the pass over keys and values, for 1086 MB without that pass.
 template <bool PACKED, bool ADD, bool REV = false>
 __global__ void __launch_bounds__(NTHR, ADD ? 3 : 2)
 la_tc_fwd_kernel(const float* __restrict__ w, const float* __restrict__ h0, int n_state, bf16* __restrict__ o, float* __restrict__ ht,
@@ -388,8 +388,11 @@ int launch_pieces(const Args& a, const Cut& cut, const CUtensorMap& map_val, con
                 reverse ? a.tok.n_seq : a.n_state, a.tok.H, cut, (int)reverse);
 }
 
-// How many parts and pieces: the least time by an estimate.  Measured: a chunk takes a CTA 4.2 us where two share an SM, 2.8 alone (backward 5.4, one to an SM), a
-// chunk of the pass over keys and values 2.6 where three do; another launch and what the parts start from 4 us.
+// How many parts and pieces: the least time by an estimate of 4.2 us for a chunk where two CTAs share an SM, 2.8 alone (backward 5.4, one to an SM), 2.6 for a
+// chunk of the pass over keys and values, and 4 for its launch and what the parts start from.  Measured are 4.5, 3.2 and (backward) 5.4 to 6, 4 where three CTAs of that
+// pass share an SM, and about one for each piece before a part's start: the estimate is low, more so for several parts.  What it is for holds: with the number of parts
+// forced, 8 to 256 units of 1000 to 16384 tokens, its choice was the fastest, or 4 % from it (128 units of 4096 tokens: 113 us in two parts, 109 in one; of
+// 16384 tokens 385 in two, 416 in one; 32 units of 16384 tokens 141 in nine, 406 in one).
 Cut cut_units(int n_seq, int max_len, int H, bool backward) {
   constexpr int SMS = 148;      // of a B200
   const int NT = (max_len + CT - 1) / CT, units = n_seq * H, slots = backward ? SMS : 2 * SMS;

@@ -7,7 +7,8 @@ Per (sequence, head), with ``S`` a matrix of value by key channels::
 The interface follows ``generalized_delta_rule``: ``w`` is the raw decay input, states are float32 ``[N, H, V, K]``, the output has
 ``r``'s dtype.  ``w`` is a number per head (``[H]``, a fixed or learned decay) or per token and head (``[B, T, H]``, a decay that depends on the
 data), and is taken in float32 whatever the tokens' dtype.  Any decay is exact: nothing is divided by a product of decays, so
-``w = -1e9`` leaves the state alone (padding) and a large ``w`` clears it (the start of another document).
+``w = -1e9`` leaves the state alone (padding) and a large ``w`` clears it (the start of another document).  Values that are not finite reach
+no other sequence and no token before the chunk they are in (128 tokens for bfloat16 at head size 64, else 64), but may reach earlier ones of it.
 
 ``linear_attention`` is the operator of prompts and training (a chunked form, forward and backward), ``linear_attention_varlen`` the same
 over sequences packed end to end, and ``LinearAttentionDecodeState`` the recurrent form for one token at a time.
