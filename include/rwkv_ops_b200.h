@@ -334,7 +334,8 @@ int rwkvb200_wkv6_bwd_varlen(const void* r, const void* k, const void* v, const 
  *   S_t = exp(-exp(w_t)) S_{t-1} + v_t k_t^T        o_t = S_t r_t        S [V][K], float32
  *   r, k, v, o   [B][T][H][D] ([B][H][T][D] when head_first), or with seq_start / seq_len (device arrays, n_seq entries)
  *                packed in one row [1][total][H][D]; then n_seq counts the sequences, max_len is the longest length, and rows
- *                of no sequence are neither read into a result nor written.  Dense: n_seq = B, max_len = T, total ignored.
+ *                of no sequence are neither read into a result nor written; an empty sequence hands its state on.  Dense: n_seq = B,
+ *                max_len = T, total ignored.
  *   w            float32: one number per head [H] (w_per_head) or per token and head, laid out like the tokens without D
  *   head size    64 or 128
  *   h0           float32 [n_state][H][D][D], n_state 0 (none: zero), 1 (shared) or n_seq;  ht [n_seq][H][D][D], may be NULL

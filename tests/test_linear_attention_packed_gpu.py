@@ -181,3 +181,80 @@ def test_a_sequence_leaves_its_neighbours_alone(name, dtype, D):
             assert torch.equal(p[[0, 1, 3]], q[[0, 1, 3]])
         else:
             assert torch.equal(p[:, :131], q[:, :131]) and torch.equal(p[:, 195:], q[:, 195:])
+
+
+@pytest.mark.parametrize("compact", [False, True])
+@pytest.mark.parametrize("dtype,D", [(F32, 64), (BF16, 64), (F16, 128)])
+def test_sequences_without_tokens(dtype, D, compact):
+    """Through the C interface a sequence may be empty: its last state is its first one, and so are their gradients."""
+    from rwkv_ops_b200 import _lib
+    lib = _lib.load()
+    start, lens, total, H, code = [0, 0, 400, 400, 401, 402, 402], [0, 400, 0, 1, 1, 0, 0], 402, 2, CODE[dtype]
+    n, full = len(lens), [i for i, m in enumerate(lens) if m]
+    x = ref.inputs(1, total, H, D, dtype=dtype, w="head", seed=37)
+    g = torch.Generator().manual_seed(38)
+    x["s0"], x["d_s"] = 0.1 * torch.randn(n, H, D, D, generator=g), 0.1 * torch.randn(n, H, D, D, generator=g)
+    want = sequences_alone({**x, "s0": x["s0"][full], "d_s": x["d_s"][full]}, [start[i] for i in full], [lens[i] for i in full], len(full))
+    a = {q: x[q].cuda() for q in ("r", "w", "k", "v", "d_o", "s0", "d_s")}
+    at, ln = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in (start, lens))
+    nan = lambda size: torch.full((max(16, size),), 0xff, dtype=torch.uint8, device="cuda")
+    out = {q: torch.empty(1, total, H, D, dtype=dtype, device="cuda") for q in ("o", "dr", "dk", "dv")}
+    out["dw"], out["s"], out["ds0"] = torch.empty(H, device="cuda"), torch.empty(n, H, D, D, device="cuda"), torch.empty(n, H, D, D, device="cuda")
+    p, sizes = (lambda t: t.data_ptr()), (n, max(lens), total, H, D, code)
+    if compact:
+        states = nan(lib.rwkvb200_linattn_packed_states_bytes(*sizes, 1))
+        ws = [nan(lib.rwkvb200_linattn_packed_workspace_bytes(*sizes, 1, backward)) for backward in (0, 1)]
+    else:
+        states = nan(lib.rwkvb200_linattn_states_bytes(n, max(lens), H, D, code, 1))
+        ws = [nan(lib.rwkvb200_linattn_workspace_bytes(*sizes, 1, backward)) for backward in (0, 1)]
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.rwkvb200_linattn_fwd(p(a["r"]), p(a["w"]), 1, p(a["k"]), p(a["v"]), p(a["s0"]), n, p(out["o"]), p(out["s"]), p(states), states.numel(),
+                                    p(ws[0]), ws[0].numel(), p(at), p(ln), n, max(lens), total, H, D, code, 0, stream) == 0
+    assert lib.rwkvb200_linattn_bwd(p(a["r"]), p(a["w"]), 1, p(a["k"]), p(a["v"]), p(a["d_o"]), p(a["d_s"]), p(states), states.numel(), p(out["dr"]),
+                                    p(out["dw"]), p(out["dk"]), p(out["dv"]), p(out["ds0"]), p(ws[1]), ws[1].numel(), p(at), p(ln), n, max(lens),
+                                    total, H, D, code, 0, stream) == 0
+    empty = [i for i in range(n) if i not in full]
+    assert torch.equal(out["s"][empty], a["s0"][empty]) and torch.equal(out["ds0"][empty], a["d_s"][empty])
+    ref.check({**out, "s": out["s"][full], "ds0": out["ds0"][full]}, want, dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_packed_calls_captured_and_at_once(dtype):
+    """One long sequence among short ones, from a graph that is replayed on other values, and from two streams at once: the same bits."""
+    import rwkv_ops_b200 as ro
+    g = torch.Generator().manual_seed(39)
+    lens, H = [5, 900, 1, 40, 7, 130, 3, 3, 60], 2
+    cu = torch.tensor([0] + lens).cumsum(0)
+    p = ro.PackedSequences(cu, "cuda")
+
+    def inputs(seed):
+        x = ref.inputs(1, int(cu[-1]), H, dtype=dtype, w="head", seed=seed)
+        x["d_s"] = 0.1 * torch.randn(len(lens), H, 64, 64, generator=g)
+        return [x[q].cuda() for q in ("r", "w", "k", "v", "d_o", "d_s")]
+
+    def call(t):
+        a = [y.detach().requires_grad_(True) for y in t[:4]]
+        o, s = ro.linear_attention_varlen(*a, p)
+        return [y.detach() for y in (o, s, *torch.autograd.grad((o, s), a, t[4:]))]
+
+    one, two = inputs(40), inputs(41)
+    want = [call(one), call(two)]
+    held = [t.clone() for t in one]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call(held)
+    for i, src in ((1, two), (0, one)):
+        for t, y in zip(held, src):
+            t.copy_(y)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, want[i]))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        both = []
+        for s, t in zip(streams, (one, two)):
+            with torch.cuda.stream(s):
+                both.append(call(t))
+        torch.cuda.synchronize()
+        for a, b in zip(both, want):
+            assert all(torch.equal(u, v) for u, v in zip(a, b))
